@@ -55,6 +55,22 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+class _Here:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        pass
+
+
+_HERE = _Here()
+
+
+def _device_of(t: torch.Tensor):
+    """Makes the tensor's device the current one around a launch, where it is not."""
+    return _HERE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.get_device())
+
+
 # ------------------------------------------------------------------------ GEMM
 # plain GEMMs of 256 x 128 and more enter at the CTA-pair kernel, which hands outputs of one wave of 128 x 128 tiles
 # to the single-CTA kernel; SS_GEMM_PAIR=0 keeps all of them on that one
@@ -464,6 +480,64 @@ def clipped_policy_(logits, targets, weights, old_logp, advantage, loss_sum, *, 
     return loss_sum
 
 
+def preference_(logits, targets, weights, cu_seqlens, loss_sum, *, beta=0.1, kind="sigmoid", label_smoothing=0.0,
+                average=False, ref_logp=None, grad_scale=1.0, write_grad=True, grad=None, sums=None, logp=None):
+    """Paired preference loss of a logits block: sequences ``2p`` and ``2p + 1`` of ``cu_seqlens`` (int32, row bounds in
+    the block) are the chosen and the rejected answer of pair ``p``. Adds the pairs' losses into ``loss_sum`` (fp32[1]) and
+    rewrites ``logits`` with their gradient (or writes it to ``grad``, of the same shape and type).
+
+    A sequence's log ratio is the sum over its rows of ``weight * (log p(target) - ref_logp)`` (``average``: divided by the
+    weights' sum; no ``ref_logp``: no reference), a pair's margin ``z`` is ``beta`` times the difference of its two, and its loss
+    ``-(1 - label_smoothing) log sigmoid(z) - label_smoothing log sigmoid(-z)`` (``"sigmoid"``), ``max(0, 1 - z)``
+    (``"hinge"``) or ``(z / beta - 1 / (2 beta))^2`` (``"ipo"``). Rows without a target in the vocabulary or with weight 0
+    count for nothing and are not read; a pair with a side of only such rows has no loss. They, and rows of no sequence,
+    get a gradient of zero. ``sums`` (fp32, one per sequence) receives the log ratios and ``logp`` (fp32[R]) the rows'
+    log-probabilities, 0 where nothing is scored."""
+    R, V = logits.shape
+    if kind not in reference.PREFERENCE_KINDS:
+        raise ValueError(f"unknown preference loss {kind!r}; known: {reference.PREFERENCE_KINDS}")
+    if not beta > 0 or not 0.0 <= label_smoothing < 1.0 or (label_smoothing and kind != "sigmoid"):
+        raise ValueError("beta is positive, label_smoothing in [0, 1) and for the sigmoid loss only")
+    S = cu_seqlens.numel() - 1
+    if cu_seqlens.dim() != 1 or cu_seqlens.dtype != torch.int32 or S < 0 or S % 2:
+        raise ValueError("cu_seqlens is int32 [2 * pairs + 1]")
+    if targets.dtype != torch.int64 or targets.shape != (R,):
+        raise ValueError("targets are int64, one per row")
+    for name, t, n in (("weights", weights, R), ("ref_logp", ref_logp, R), ("logp", logp, R), ("sums", sums, S),
+                       ("loss_sum", loss_sum, 1)):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous()):
+            raise ValueError(f"{name} is contiguous fp32 [{n}]")
+    if grad is not None and (grad.shape != logits.shape or grad.dtype != logits.dtype):
+        raise ValueError("grad has the logits' shape and type")
+    if any(t is not None and t.device != logits.device
+           for t in (targets, weights, cu_seqlens, loss_sum, ref_logp, grad, sums, logp)):
+        raise ValueError("all tensors of a preference loss are on one device")
+    out = (logits if grad is None else grad) if write_grad else None
+    if not _cuda(logits):
+        loss, s, lp = reference.preference_(logits, targets, weights, cu_seqlens, beta, kind, label_smoothing, average,
+                                            ref_logp, grad_scale, out)
+        loss_sum.add_(loss)
+        if sums is not None:
+            sums.copy_(s)
+        if logp is not None:
+            logp.copy_(lp)
+        return loss_sum
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError("preference logits are bf16 or fp32 on CUDA")
+    if logits.stride(1) != 1 or (out is not None and out.stride(1) != 1) or not (targets.is_contiguous() and cu_seqlens.is_contiguous()):
+        raise ValueError("logits and their gradient have unit inner stride, targets and cu_seqlens are contiguous")
+    with _device_of(logits):
+        work = torch.empty(4 * R + S // 2 + 1, dtype=torch.float32, device=logits.device)
+        lp = torch.empty(R, dtype=torch.float32, device=logits.device) if logp is None else logp
+        _lib.check(_lib.lib().ss_preference(
+            logits.data_ptr(), int(logits.dtype == torch.float32), max(logits.stride(0), V), targets.data_ptr(), _ptr(weights),
+            cu_seqlens.data_ptr(), R, V, S // 2, _ptr(ref_logp), float(beta), reference.PREFERENCE_KINDS.index(kind),
+            float(label_smoothing), int(average), float(grad_scale), lp.data_ptr(), _ptr(sums), loss_sum.data_ptr(), _ptr(out),
+            0 if out is None else max(out.stride(0), V), work.data_ptr(), _lib.stream_ptr()),
+            "ss_preference" if out is None else "ss_preference with its gradient")
+    return loss_sum
+
+
 def target_logprobs_(logits, targets, logp):
     """log p(target) per row of a logits block into ``logp`` (fp32[R]); logits unchanged."""
     if not _cuda(logits):
@@ -535,6 +609,70 @@ def _adamw_table(table, h):
         (ctypes.c_longlong * len(table))(*table), k, h["lr"], h["beta1"], h["beta2"], h["eps"], h["weight_decay"],
         h["step"], h["grad_scale"], h["seed"], int(h["stochastic_param"]), int(h["stochastic_state"]),
         _lib.stream_ptr()), "ss_adamw_sr_many")
+
+
+def moments8(n, device=None):
+    """Zero 8-bit moments of ``n`` elements: ``(m, r, m_exp, r_exp)``, e4m3 codes of the first moment and of the root of
+    the second, and the biased exponents (uint8) of their blocks of ``reference.MOMENT_BLOCK`` elements."""
+    blocks = -(-n // reference.MOMENT_BLOCK)
+    return (torch.zeros(n, dtype=torch.float8_e4m3fn, device=device), torch.zeros(n, dtype=torch.float8_e4m3fn, device=device),
+            torch.zeros(blocks, dtype=torch.uint8, device=device), torch.zeros(blocks, dtype=torch.uint8, device=device))
+
+
+def _check_moments8(p, g, m, r, m_exp, r_exp, offset):
+    n = p.numel()
+    blocks = -(-n // reference.MOMENT_BLOCK)
+    if g.numel() != n or m.numel() != n or r.numel() != n or m_exp.numel() != blocks or r_exp.numel() != blocks:
+        raise ValueError(f"a parameter of {n} elements has a gradient and codes of as many and {blocks} exponents per moment")
+    if m.dtype != torch.float8_e4m3fn or r.dtype != torch.float8_e4m3fn or m_exp.dtype != torch.uint8 or r_exp.dtype != torch.uint8:
+        raise TypeError("8-bit moments are float8_e4m3fn codes with uint8 exponents (moments8)")
+    for t in (p, g):
+        if t.dtype != torch.float32 and t.dtype != _BF16:
+            raise TypeError("parameters and gradients with 8-bit moments are bf16 or fp32")
+    for t in (p, g, m, r, m_exp, r_exp):
+        if not t.is_contiguous() or t.device != p.device:
+            raise ValueError("a parameter, its gradient and its moments are contiguous and on one device")
+    if offset < 0 or offset % 8:
+        raise ValueError("offsets are multiples of 8")
+
+
+def adamw8_many_(tensors, *, lr, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.0, step=1, grad_scale=1.0, seed=0,
+                 stochastic_param=True, stochastic_state=True):
+    """AdamW with 8-bit moments for every ``(p, g, m, r, m_exp, r_exp, offset)`` (``moments8`` makes the last but one four),
+    in shared launches. ``p`` and ``g`` are bf16 or fp32. The moments take 2 bytes and 1/128 an element (4 in bf16) and are
+    rounded stochastically, like bf16 parameters, by a counter RNG keyed on (seed, step, offset + element), or to nearest;
+    moments rounded to nearest stop following a gradient whose size changes by less than a code's step. A tensor may be updated
+    in parts that start on whole blocks, with the same bits. On the CPU all roundings are to nearest."""
+    if step < 1:
+        raise ValueError("steps count from 1")
+    hyper = dict(lr=lr, beta1=beta1, beta2=beta2, eps=eps, weight_decay=weight_decay, step=step, grad_scale=grad_scale)
+    tables: dict = {}                       # (device, types) -> (a tensor there, eight numbers a tensor); insertion-ordered
+    seen = set()
+
+    def flush():
+        for (_, p_dtype, g_dtype), (where, table) in tables.items():
+            with _device_of(where):
+                _lib.check(_lib.lib().ss_adamw8_many(
+                    (ctypes.c_longlong * len(table))(*table), len(table) // 8, int(p_dtype == torch.float32),
+                    int(g_dtype == torch.float32), lr, beta1, beta2, eps, weight_decay, step, grad_scale, seed,
+                    int(stochastic_param), int(stochastic_state), _lib.stream_ptr()), "ss_adamw8_many")
+        tables.clear()
+        seen.clear()
+
+    for p, g, m, r, m_exp, r_exp, offset in tensors:
+        _check_moments8(p, g, m, r, m_exp, r_exp, offset)
+        if not _cuda(p):
+            reference.adamw8_(p, g, m, r, m_exp, r_exp, **hyper)
+            continue
+        at, n = p.data_ptr(), p.numel()
+        if n == 0:
+            continue
+        if at in seen:                      # a parameter listed twice is updated twice, in order
+            flush()
+        seen.add(at)
+        tables.setdefault((p.get_device(), p.dtype, g.dtype), (p, []))[1].extend(
+            (at, g.data_ptr(), m.data_ptr(), r.data_ptr(), m_exp.data_ptr(), r_exp.data_ptr(), n, offset))
+    flush()
 
 
 def sumsq(x, partials, out, accumulate=False):

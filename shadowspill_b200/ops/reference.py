@@ -294,3 +294,146 @@ def router_topk(logits, top_k, renormalize=True):
         w = torch.softmax(logits.float(), dim=-1).gather(1, ids)
     counts = torch.bincount(ids.reshape(-1), minlength=logits.shape[-1])
     return w, ids, counts
+
+
+def expert_scores(logits, scoring):
+    """Scores in the logits' precision: ``sigmoid``, or a softmax in which a row of -inf has scores of zero."""
+    if scoring == "sigmoid":
+        return torch.sigmoid(logits)
+    top = logits.amax(-1, keepdim=True)
+    e = torch.exp(logits - torch.where(top == float("-inf"), torch.zeros_like(top), top))
+    return e / e.sum(-1, keepdim=True).clamp(min=1.0)
+
+
+def select_experts(logits, k, scoring="softmax", bias=None, groups=1, keep_groups=1, renormalize=True, scale=1.0):
+    """Definition of :func:`..routing.select_experts`: keys in 64 bits, ties to the lowest index, experts without a
+    comparable key last. Returns (ids int32 [T,k], weights fp32 [T,k], counts int32 [E])."""
+    T, E = logits.shape
+    x = logits.double()
+    s = expert_scores(x, scoring)
+    key = x if bias is None and groups == 1 else s if bias is None else s + bias.double()
+    key = torch.where(torch.isnan(key), torch.full_like(key, float("-inf")), key)
+    if groups > 1:
+        g = key.view(T, groups, E // groups)
+        best = torch.sort(g, dim=-1, descending=True).values[..., :2].sum(-1)
+        kept = torch.sort(best, dim=-1, descending=True, stable=True).indices[:, :keep_groups]
+        drop = torch.ones(T, groups, dtype=torch.bool, device=x.device).scatter_(1, kept, False)
+        key = g.masked_fill(drop[..., None], float("-inf")).reshape(T, E)
+    ids = torch.sort(key, dim=-1, descending=True, stable=True).indices[:, :k]
+    w = s.gather(1, ids)
+    if renormalize:
+        w = w / (w.sum(-1, keepdim=True) + 1e-20)
+    counts = torch.zeros(E, dtype=torch.int32, device=x.device)
+    counts.index_add_(0, ids.reshape(-1), torch.ones(T * k, dtype=torch.int32, device=x.device))
+    return ids.to(torch.int32), (w * scale).float(), counts
+
+
+def select_experts_bwd(logits, ids, dweights, scoring="softmax", renormalize=True, scale=1.0):
+    """Gradient of the weights of :func:`select_experts` with respect to the logits, the picks held fixed."""
+    s = expert_scores(logits.double(), scoring)
+    at = ids.long()
+    c, dw = s.gather(1, at), dweights.double()
+    dc = scale * dw
+    if renormalize:
+        total = c.sum(-1, keepdim=True) + 1e-20
+        dc = (dc - (dc * c / total).sum(-1, keepdim=True)) / total
+    wide = torch.zeros_like(s).scatter_(1, at, dc)
+    dx = wide * s * (1 - s) if scoring == "sigmoid" else s * (wide - (dc * c).sum(-1, keepdim=True))
+    return dx.to(logits.dtype)
+
+
+PREFERENCE_KINDS = ("sigmoid", "hinge", "ipo")
+
+
+def preference_terms(sums, beta, kind, label_smoothing):
+    """Loss of each pair and its derivative by ``sums[2i]`` (that by ``sums[2i + 1]`` is the negative), from the
+    sequences' log ratios."""
+    z = beta * (sums[0::2] - sums[1::2])
+    if kind == "sigmoid":
+        loss = (1 - label_smoothing) * F.softplus(-z) + label_smoothing * F.softplus(z)
+        slope = beta * (label_smoothing - torch.sigmoid(-z))
+    elif kind == "hinge":
+        loss, slope = torch.relu(1 - z), torch.where(z < 1, -beta, 0.0).to(z.dtype)
+    else:
+        gap = sums[0::2] - sums[1::2] - 1 / (2 * beta)
+        loss, slope = gap * gap, 2 * gap
+    return loss, slope
+
+
+def preference_(logits, targets, weights, cu_seqlens, beta, kind, label_smoothing, average, ref_logp, grad_scale, grad):
+    """Paired preference loss over a logits block, sums and coefficients in 64 bits; ``grad`` (when given) receives the
+    gradient. Returns (loss fp32 scalar, sums fp32[S], logp fp32[R])."""
+    R, V = logits.shape
+    f = logits.float()
+    w = torch.ones(R, device=f.device) if weights is None else weights.float()
+    valid = (targets >= 0) & (targets < V) & (w != 0)
+    t = torch.where(valid, targets, torch.zeros_like(targets))[:, None]
+    logp = torch.where(valid, f.gather(1, t)[:, 0] - torch.logsumexp(f, -1), torch.zeros_like(w))
+    ratio = logp if ref_logp is None else logp - ref_logp.float()
+    ratio = torch.where(valid, w * ratio, torch.zeros_like(w)).double()
+    bounds = [min(max(int(c), 0), R) for c in cu_seqlens.tolist()]
+    spans = [(a, max(a, b)) for a, b in zip(bounds[:-1], bounds[1:])]
+    sums = torch.stack([ratio[a:b].sum() for a, b in spans]) if spans else ratio.new_zeros(0)
+    mass = torch.stack([torch.where(valid, w, 0.0)[a:b].double().sum() for a, b in spans]) if spans else ratio.new_zeros(0)
+    some = torch.tensor([bool(valid[a:b].any()) for a, b in spans], dtype=torch.bool, device=f.device)
+    if average:
+        sums = torch.where(mass != 0, sums / mass, torch.zeros_like(sums))
+    loss, slope = preference_terms(sums, beta, kind, label_smoothing)
+    live = some[0::2] & some[1::2]
+    loss = torch.where(live, loss, torch.zeros_like(loss)).sum()
+    if grad is not None:
+        slope = torch.where(live, slope, torch.zeros_like(slope))
+        coef = torch.zeros(R, dtype=torch.float64, device=f.device)
+        for i, (a, b) in enumerate(spans):
+            each = slope[i // 2] * (1 - 2 * (i % 2))
+            if average:
+                each = torch.where(mass[i] != 0, each / mass[i], torch.zeros_like(each))
+            coef[a:b] = torch.where(valid[a:b], w[a:b].double() * each, 0.0)
+        coef = (coef * grad_scale).float()
+        onehot = torch.zeros_like(f).scatter_(1, t, 1.0)
+        full = (onehot - torch.softmax(f, -1)) * coef[:, None]
+        grad.copy_(torch.where(valid[:, None], full, torch.zeros_like(full)).to(grad.dtype))
+    return loss.float(), sums.float(), logp
+
+
+MOMENT_BLOCK = 256        # elements that share the exponent of an 8-bit moment
+
+
+def moment_exponents(top):
+    """Biased exponents of the smallest powers of two with ``top <= 448 * 2^(e - 127)``, 0 for blocks of zeros."""
+    bits = top.contiguous().view(torch.int32)
+    e = (bits >> 23) - torch.where((bits & 0x7fffff) > 0x600000, 7, 8)
+    return torch.where(top > 0, e.clamp(1, 254), torch.zeros_like(e)).to(torch.uint8)
+
+
+def moment_values(codes, exponents):
+    """What 8-bit moments stand for, in fp32."""
+    unit = torch.exp2(exponents.float() - 127.0).repeat_interleave(MOMENT_BLOCK)[:codes.numel()]
+    return codes.float() * unit
+
+
+def moment_codes(x, floor=False):
+    """fp32 values -> (e4m3 codes, exponents); with ``floor`` a value that is not zero keeps a code that is not."""
+    n = x.numel()
+    blocks = F.pad(x, (0, -n % MOMENT_BLOCK)).view(-1, MOMENT_BLOCK)
+    e = moment_exponents(torch.where(torch.isnan(blocks), 0.0, blocks.abs()).amax(1) if n else x.new_zeros(0))
+    y = (blocks * torch.exp2(127.0 - e.float())[:, None]).reshape(-1)[:n]
+    if floor:
+        y = torch.where(x > 0, y.clamp(min=2.0 ** -9), y)
+    return y.clamp(-448.0, 448.0).to(torch.float8_e4m3fn), e
+
+
+def adamw8_(p, g, m, r, m_exp, r_exp, *, lr, beta1, beta2, eps, weight_decay, step, grad_scale=1.0):
+    """Round-to-nearest AdamW with 8-bit moments (in place): ``m`` and ``r``, the root of the second moment, as e4m3
+    codes with an exponent per block. The moments' arithmetic is fp32, one rounding to an operation."""
+    gf = g.float() * grad_scale
+    mf = beta1 * moment_values(m, m_exp) + (1 - beta1) * gf
+    old = moment_values(r, r_exp)
+    rf = torch.sqrt(beta2 * (old * old) + (1 - beta2) * gf * gf)
+    pf = p.float() * (1 - lr * weight_decay)
+    pf = pf - lr * (mf / (1 - beta1 ** step)) / (rf / math.sqrt(1 - beta2 ** step) + eps)
+    p.copy_(pf.to(p.dtype))
+    for codes, exps, x, floor in ((m, m_exp, mf, False), (r, r_exp, rf, True)):
+        c, e = moment_codes(x, floor)
+        codes.copy_(c)
+        exps.copy_(e)
