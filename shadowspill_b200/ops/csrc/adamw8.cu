@@ -28,15 +28,15 @@ struct Tensor8 {
   uint8_t *m, *r, *m_exp, *r_exp;
   long long n;
   unsigned long long offset;   // global element offset of the range: what the random bits are drawn by
-  int first;                   // the launch's first run of this tensor
+  int first;                   // the launch's first CTA of this tensor
   int vectors;                 // are all pointers on the boundaries of their 8-element pieces?
 };
 struct Table8 {
   Tensor8 t[A8_TENSORS];
-  int count, run;              // run: blocks that a warp walks
+  int count, run;              // run: blocks that each warp of a CTA walks
 };
 struct Args8 {
-  float lr, beta1, beta2, c1, c2, eps, keep, inv_bias1, inv_bias2, grad_scale;
+  float beta1, beta2, c1, c2, eps, keep, minus_lr, inv_bias2, grad_scale, one;   // minus_lr: with the first bias correction
   unsigned long long seed;
 };
 
@@ -53,58 +53,94 @@ __device__ __forceinline__ uint4 philox(uint4 c, uint2 key) {
   return c;
 }
 
-__device__ __forceinline__ void decode8(uint2 codes, float unit, float (&f)[8]) {
+// The eight elements of a lane, by pairs: two fp32 operations to an instruction. Each operation is rounded by itself.
+struct Eight {
+  float2 v[4];
+};
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+// A sum of two rounded products by itself: packed products and sums are joined to fused multiply-adds, which round once,
+// whatever their spelling, so the sum is spelled a * one + b with a `one` that the compiler does not know.
+__device__ __forceinline__ float2 add2(float2 a, float2 b, float one) { return __ffma2_rn(a, both(one), b); }
+
+__device__ __forceinline__ void decode8(uint2 codes, float unit, Eight& out) {
   const uint32_t w[2] = {codes.x, codes.y};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i >> 1] >> (16 * (i & 1))), __NV_E4M3);
-    const float2 v = __half22float2(__half2(h));
-    f[2 * i] = v.x * unit;
-    f[2 * i + 1] = v.y * unit;
+    out.v[i] = __fmul2_rn(__half22float2(__half2(h)), both(unit));
   }
 }
 // Eight scaled values -> codes, to nearest or by eight random bits each.
-template <bool SR>
-__device__ __forceinline__ uint2 encode8(const float (&f)[8], uint32_t r0, uint32_t r1) {
-  uint2 out;
-  if (SR) {
-    asm("cvt.rs.satfinite.e4m3x4.f32 %0, {%1, %2, %3, %4}, %5;"
-        : "=r"(out.x) : "f"(f[3]), "f"(f[2]), "f"(f[1]), "f"(f[0]), "r"(r0));
-    asm("cvt.rs.satfinite.e4m3x4.f32 %0, {%1, %2, %3, %4}, %5;"
-        : "=r"(out.y) : "f"(f[7]), "f"(f[6]), "f"(f[5]), "f"(f[4]), "r"(r1));
-  } else {
-    uint32_t w[4];
+__device__ __forceinline__ uint2 encode8(const Eight& f) {
+  uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * i], f[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
-    out = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
-  }
+  for (int i = 0; i < 4; ++i) w[i] = __nv_cvt_float2_to_fp8x2(f.v[i], __NV_SATFINITE, __NV_E4M3);
+  return make_uint2(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410));
+}
+__device__ __forceinline__ uint2 encode8(const Eight& f, uint32_t r0, uint32_t r1) {
+  uint2 out;
+  asm("cvt.rs.satfinite.e4m3x4.f32 %0, {%1, %2, %3, %4}, %5;"
+      : "=r"(out.x) : "f"(f.v[1].y), "f"(f.v[1].x), "f"(f.v[0].y), "f"(f.v[0].x), "r"(r0));
+  asm("cvt.rs.satfinite.e4m3x4.f32 %0, {%1, %2, %3, %4}, %5;"
+      : "=r"(out.y) : "f"(f.v[3].y), "f"(f.v[3].x), "f"(f.v[2].y), "f"(f.v[2].x), "r"(r1));
   return out;
 }
-// Biased exponent of the block whose largest magnitude is `top` (this lane's; the warp's is meant). 448 = 1.75 * 2^8.
-__device__ __forceinline__ int block_exponent(float top) {
-  const unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+// Biased exponent of a block whose largest magnitude has these bits. 448 = 1.75 * 2^8.
+__device__ __forceinline__ int block_exponent(unsigned bits) {
   if (bits == 0) return 0;
   const int e = static_cast<int>(bits >> 23) - ((bits & 0x7fffffu) > 0x600000u ? 7 : 8);
   return e > 1 ? e : 1;
 }
-
-template <class T> __device__ __forceinline__ float one(const T* x, long long i);
-template <> __device__ __forceinline__ float one(const float* x, long long i) { return x[i]; }
-template <> __device__ __forceinline__ float one(const bf16* x, long long i) { return __bfloat162float(x[i]); }
-template <class T> __device__ __forceinline__ void load8(const T* x, float (&f)[8]);
-template <> __device__ __forceinline__ void load8(const float* x, float (&f)[8]) {
-  const float4 a = reinterpret_cast<const float4*>(x)[0], b = reinterpret_cast<const float4*>(x)[1];
-  f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+__device__ __forceinline__ float unit_of(int exponent) { return __uint_as_float(static_cast<uint32_t>(exponent) << 23); }
+__device__ __forceinline__ unsigned warp_top(float lane_top) { return __reduce_max_sync(0xffffffffu, __float_as_uint(lane_top)); }
+__device__ __forceinline__ float sqrt_near(float x) {
+  float y;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
-template <> __device__ __forceinline__ void load8(const bf16* x, float (&f)[8]) {
-  const uint4 u = *reinterpret_cast<const uint4*>(x);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+__device__ __forceinline__ float reciprocal_near(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float largest(const Eight& f) {
+  float t = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
+  for (int i = 0; i < 4; ++i) t = fmaxf(t, fmaxf(fabsf(f.v[i].x), fabsf(f.v[i].y)));
+  return t;
 }
+
+// What a lane reads of a block.
+template <class T> struct Piece8;
+template <> struct Piece8<bf16> {
+  uint4 u;
+  __device__ __forceinline__ void load(const uint4* x) { u = x[0]; }
+  __device__ __forceinline__ void set(int e, bf16 x) {
+    reinterpret_cast<unsigned short*>(&u)[e] = __bfloat16_as_ushort(x);
+  }
+  __device__ __forceinline__ void get(Eight& f) const {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f.v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+  }
+};
+template <> struct Piece8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const uint4* x) {
+    a = *reinterpret_cast<const float4*>(x);
+    b = *reinterpret_cast<const float4*>(x + 32);
+  }
+  __device__ __forceinline__ void set(int e, float x) { (e < 4 ? reinterpret_cast<float*>(&a) : reinterpret_cast<float*>(&b))[e & 3] = x; }
+  __device__ __forceinline__ void get(Eight& f) const {
+    f.v[0] = make_float2(a.x, a.y); f.v[1] = make_float2(a.z, a.w); f.v[2] = make_float2(b.x, b.y); f.v[3] = make_float2(b.z, b.w);
+  }
+};
+template <class P, class G> struct Read8 {
+  Piece8<P> p;
+  Piece8<G> g;
+  uint2 m, r;
+  int m_exp, r_exp;
+};
 
 // fp32 -> bf16 bits: to nearest, or 16 random bits below the kept mantissa and a cut (inf and NaN are only cut).
 template <bool SR>
@@ -114,110 +150,224 @@ __device__ __forceinline__ uint32_t bf16_bits(float f, uint32_t rnd16) {
   return ((u & 0x7f800000u) == 0x7f800000u ? u : u + rnd16) >> 16;
 }
 
+// One block of 256 elements, eight to a lane: `x` becomes what is written, the parameters as fp32 in `p`.
+//
+// The root is needed as its code and for the parameter's step. sqrt.approx (relative error 2^-23) gives both, unless
+// its value lies within 2^-21 of a border between two codes, where it is taken again with a correct rounding: that is one
+// element in 30,000. So it is for a block whose exponent is in doubt, and for one with roots so small that their squares
+// lose bits. (With the correctly rounded root everywhere: +10 instructions an element.)
+template <bool SR_PARAM, bool SR_STATE, class P, class G>
+__device__ __forceinline__ void update8(Read8<P, G>& x, const Args8& a, unsigned long long element, Eight& p, uint4& random) {
+  Eight g, m, v, r;
+  x.p.get(p);
+  x.g.get(g);
+  decode8(x.m, unit_of(x.m_exp), m);
+  decode8(x.r, unit_of(x.r_exp), r);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 gg = __fmul2_rn(g.v[i], both(a.grad_scale));
+    m.v[i] = add2(__fmul2_rn(both(a.beta1), m.v[i]), __fmul2_rn(both(a.c1), gg), a.one);
+    v.v[i] = add2(__fmul2_rn(both(a.beta2), __fmul2_rn(r.v[i], r.v[i])), __fmul2_rn(__fmul2_rn(both(a.c2), gg), gg), a.one);
+    r.v[i] = make_float2(sqrt_near(v.v[i].x), sqrt_near(v.v[i].y));
+  }
+  auto exact_roots = [&] {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.v[i] = make_float2(__fsqrt_rn(v.v[i].x), __fsqrt_rn(v.v[i].y));
+  };
+  x.m_exp = block_exponent(warp_top(largest(m)));
+  unsigned top = warp_top(largest(r));
+  const unsigned off = (top & 0x7fffffu) - 0x5ffffcu;          // four steps to either side of the border
+  if (top < 0x2b800000u || (!SR_STATE && off <= 8u)) {         // 2^-40
+    exact_roots();
+    top = warp_top(largest(r));
+  }
+  x.r_exp = block_exponent(top);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 d = __ffma2_rn(r.v[i], both(a.inv_bias2), both(a.eps));
+    const float2 step = __fmul2_rn(m.v[i], both(a.minus_lr));
+    p.v[i] = __ffma2_rn(step, make_float2(reciprocal_near(d.x), reciprocal_near(d.y)), __fmul2_rn(p.v[i], both(a.keep)));
+  }
+  uint4 rs = make_uint4(0, 0, 0, 0);
+  if (SR_PARAM || SR_STATE) {
+    const unsigned long long at = element >> 3;
+    const uint2 key = make_uint2(static_cast<uint32_t>(a.seed), static_cast<uint32_t>(a.seed >> 32));
+    const uint32_t c0 = static_cast<uint32_t>(at), c1 = static_cast<uint32_t>(at >> 32);
+    if (SR_PARAM) random = philox(make_uint4(c0, c1, 0u, 0x3838u), key);
+    if (SR_STATE) rs = philox(make_uint4(c0, c1, 1u, 0x3838u), key);
+  }
+  const float m_inv = unit_of(254 - x.m_exp), r_inv = unit_of(254 - x.r_exp);
+  constexpr float FLOOR = 0.001953125f;                        // code 1
+  auto scaled = [&](Eight& out) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 y = __fmul2_rn(r.v[i], both(r_inv));
+      out.v[i] = make_float2(v.v[i].x > 0.f ? fmaxf(y.x, FLOOR) : y.x, v.v[i].y > 0.f ? fmaxf(y.y, FLOOR) : y.y);
+    }
+  };
+  Eight y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m.v[i] = __fmul2_rn(m.v[i], both(m_inv));
+  scaled(y);
+  if (SR_STATE) {
+    x.m = encode8(m, rs.x, rs.y);
+    x.r = encode8(y, rs.z, rs.w);
+  } else {
+    x.m = encode8(m);
+    Eight low, high;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      low.v[i] = __fmul2_rn(y.v[i], both(1.f - 0x1p-21f));
+      high.v[i] = __fmul2_rn(y.v[i], both(1.f + 0x1p-21f));
+    }
+    x.r = encode8(low);
+    const uint2 other = encode8(high);
+    if (x.r.x != other.x || x.r.y != other.y) {
+      exact_roots();
+      scaled(y);
+      x.r = encode8(y);
+    }
+  }
+}
+
+__device__ __forceinline__ void copy16(const void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy8(const void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
+
+// A warp walks `run` blocks, a CTA's eight warps side by side. Blocks to come are on their way in shared memory, where a lane reads
+// only what it asked for itself, so nothing but its own copies is waited for. (With the next block in registers instead the
+// compiler moves the loads down to their use for want of registers: 218 M elements 668 us.)
+template <class P, class G> struct Ring8 {
+  static constexpr int P16 = sizeof(P) / 2, G16 = sizeof(G) / 2;       // 16-byte pieces of a lane
+  static constexpr int STAGE = 32 * (16 * P16 + 16 * G16 + 16), STAGES = 48 * 1024 / A8_WARPS / STAGE;
+};
 template <class P, class G, bool SR_PARAM, bool SR_STATE>
-__global__ void __launch_bounds__(A8_THREADS)
+__global__ void __launch_bounds__(A8_THREADS, 3)
 adamw8_kernel(const __grid_constant__ Table8 tab, Args8 a) {
-  const int lane = threadIdx.x & 31, run = blockIdx.x * A8_WARPS + (threadIdx.x >> 5);
-  int lo = 0, hi = tab.count - 1;                // the last tensor that starts at or before this run
+  using Ring = Ring8<P, G>;
+  __shared__ __align__(16) unsigned char ring[A8_WARPS][Ring::STAGES][Ring::STAGE];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int lo = 0, hi = tab.count - 1;                // the last tensor that starts at or before this CTA
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (tab.t[mid].first <= run) lo = mid; else hi = mid - 1;
+    if (tab.t[mid].first <= static_cast<int>(blockIdx.x)) lo = mid; else hi = mid - 1;
   }
-  const Tensor8& t = tab.t[lo];
+  const Tensor8 t = tab.t[lo];
   P* const p = static_cast<P*>(t.p);
   const G* const g = static_cast<const G*>(t.g);
-  const long long blocks = (t.n + A8_BLOCK - 1) / A8_BLOCK, from = static_cast<long long>(run - t.first) * tab.run;
-  const long long to = from + tab.run < blocks ? from + tab.run : blocks;
-  for (long long b = from; b < to; ++b) {
-    const long long e0 = b * A8_BLOCK + lane * 8;
-    const bool whole = t.vectors && (b + 1) * A8_BLOCK <= t.n;
-    float pf[8], gf[8], mf[8], rf[8];
-    const float m_unit = __uint_as_float(static_cast<uint32_t>(t.m_exp[b]) << 23);
-    const float r_unit = __uint_as_float(static_cast<uint32_t>(t.r_exp[b]) << 23);
-    uint2 mc = make_uint2(0, 0), rc = make_uint2(0, 0);
-    if (whole) {
-      load8(p + e0, pf);
-      load8(g + e0, gf);
-      mc = *reinterpret_cast<const uint2*>(t.m + e0);
-      rc = *reinterpret_cast<const uint2*>(t.r + e0);
-    } else {
+  const long long first = static_cast<long long>(blockIdx.x - t.first) * tab.run * A8_WARPS + warp;
+  const long long blocks = (t.n + A8_BLOCK - 1) / A8_BLOCK, whole = t.vectors ? t.n / A8_BLOCK : 0;
+  auto walked = [&](long long end) {             // blocks of this warp's run before `end`
+    const long long n = first < end ? (end - first + A8_WARPS - 1) / A8_WARPS : 0;
+    return n < tab.run ? static_cast<int>(n) : tab.run;
+  };
+  const int mine = walked(blocks), full = walked(whole);
+  // the exponents of all blocks of the run, one to a lane
+  const long long kept = first + static_cast<long long>(lane) * A8_WARPS;
+  int m_exp = lane < mine ? t.m_exp[kept] : 0, r_exp = lane < mine ? t.r_exp[kept] : 0;
+  auto fetch = [&](int i) {
+    if (i < full) {
+      const long long e0 = (first + static_cast<long long>(i) * A8_WARPS) * A8_BLOCK + lane * 8;
+      uint4* q = reinterpret_cast<uint4*>(ring[warp][i % Ring::STAGES]) + lane;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const bool in = e0 + e < t.n;
-        pf[e] = in ? one(p, e0 + e) : 0.f;
-        gf[e] = in ? one(g, e0 + e) : 0.f;
-        const uint32_t m = in ? t.m[e0 + e] : 0, r = in ? t.r[e0 + e] : 0;
-        (e < 4 ? mc.x : mc.y) |= m << (8 * (e & 3));
-        (e < 4 ? rc.x : rc.y) |= r << (8 * (e & 3));
-      }
+      for (int k = 0; k < Ring::P16; ++k) copy16(q + 32 * k, reinterpret_cast<const uint4*>(p + e0) + k);
+      q += 32 * Ring::P16;
+#pragma unroll
+      for (int k = 0; k < Ring::G16; ++k) copy16(q + 32 * k, reinterpret_cast<const uint4*>(g + e0) + k);
+      uint2* c = reinterpret_cast<uint2*>(q - lane + 32 * Ring::G16) + lane;
+      copy8(c, t.m + e0);
+      copy8(c + 32, t.r + e0);
     }
-    decode8(mc, m_unit, mf);
-    decode8(rc, r_unit, rf);
-    float m_top = 0.f, r_top = 0.f;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  Eight out;
+  uint4 random;
+  Read8<P, G> x = {};
+  for (int i = 0; i < Ring::STAGES - 1; ++i) fetch(i);
+  int i = 0;
+  for (; i < full; ++i) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(Ring::STAGES - 2) : "memory");
+    const long long e0 = (first + static_cast<long long>(i) * A8_WARPS) * A8_BLOCK + lane * 8;
+    const uint4* q = reinterpret_cast<const uint4*>(ring[warp][i % Ring::STAGES]) + lane;
+    x.p.load(q);
+    q += 32 * Ring::P16;
+    x.g.load(q);
+    const uint2* c = reinterpret_cast<const uint2*>(q - lane + 32 * Ring::G16) + lane;
+    x.m = c[0];
+    x.r = c[32];
+    x.m_exp = __shfl_sync(0xffffffffu, m_exp, i);
+    x.r_exp = __shfl_sync(0xffffffffu, r_exp, i);
+    fetch(i + Ring::STAGES - 1);                 // into the stage of the block before this one
+    update8<SR_PARAM, SR_STATE>(x, a, t.offset + static_cast<unsigned long long>(e0), out, random);
+    if (sizeof(P) == 4) {
+      float4* to4 = reinterpret_cast<float4*>(p + e0);
+      to4[0] = make_float4(out.v[0].x, out.v[0].y, out.v[1].x, out.v[1].y);
+      to4[1] = make_float4(out.v[2].x, out.v[2].y, out.v[3].x, out.v[3].y);
+    } else {
+      const uint32_t rw[4] = {random.x, random.y, random.z, random.w};
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (SR_PARAM) {
+          w[k] = bf16_bits<true>(out.v[k].x, rw[k] & 0xffffu) | bf16_bits<true>(out.v[k].y, rw[k] >> 16) << 16;
+        } else {
+          const __nv_bfloat162 two = __float22bfloat162_rn(out.v[k]);
+          w[k] = *reinterpret_cast<const uint32_t*>(&two);
+        }
+      }
+      *reinterpret_cast<uint4*>(p + e0) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    *reinterpret_cast<uint2*>(t.m + e0) = x.m;
+    *reinterpret_cast<uint2*>(t.r + e0) = x.r;
+    if (lane == i) {
+      m_exp = x.m_exp;
+      r_exp = x.r_exp;
+    }
+  }
+  for (; i < mine; ++i) {                        // a tensor's last block, or one off the boundaries of the pieces
+    const long long e0 = (first + static_cast<long long>(i) * A8_WARPS) * A8_BLOCK + lane * 8;
+    x.m = x.r = make_uint2(0, 0);
+    x.m_exp = __shfl_sync(0xffffffffu, m_exp, i);
+    x.r_exp = __shfl_sync(0xffffffffu, r_exp, i);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float gg = __fmul_rn(gf[e], a.grad_scale);
-      mf[e] = __fadd_rn(__fmul_rn(a.beta1, mf[e]), __fmul_rn(a.c1, gg));
-      rf[e] = __fsqrt_rn(__fadd_rn(__fmul_rn(a.beta2, __fmul_rn(rf[e], rf[e])), __fmul_rn(__fmul_rn(a.c2, gg), gg)));
-      m_top = fmaxf(m_top, fabsf(mf[e]));
-      r_top = fmaxf(r_top, rf[e]);
-      pf[e] = pf[e] * a.keep - a.lr * __fdividef(mf[e] * a.inv_bias1, rf[e] * a.inv_bias2 + a.eps);
+      const bool in = e0 + e < t.n;
+      x.p.set(e, in ? p[e0 + e] : P(0.f));
+      x.g.set(e, in ? g[e0 + e] : G(0.f));
+      const uint32_t m = in ? t.m[e0 + e] : 0, r = in ? t.r[e0 + e] : 0;
+      (e < 4 ? x.m.x : x.m.y) |= m << (8 * (e & 3));
+      (e < 4 ? x.r.x : x.r.y) |= r << (8 * (e & 3));
     }
-    const int m_exp = block_exponent(m_top), r_exp = block_exponent(r_top);
-    const float m_inv = __uint_as_float(static_cast<uint32_t>(254 - m_exp) << 23);
-    const float r_inv = __uint_as_float(static_cast<uint32_t>(254 - r_exp) << 23);
+    update8<SR_PARAM, SR_STATE>(x, a, t.offset + static_cast<unsigned long long>(e0), out, random);
+    const uint32_t rw[4] = {random.x, random.y, random.z, random.w};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      mf[e] *= m_inv;
-      rf[e] = rf[e] > 0.f ? fmaxf(rf[e] * r_inv, 0.001953125f) : rf[e];
+      if (e0 + e >= t.n) continue;
+      const float f = (e & 1) ? out.v[e >> 1].y : out.v[e >> 1].x;
+      if (sizeof(P) == 4) reinterpret_cast<float*>(p)[e0 + e] = f;
+      else reinterpret_cast<unsigned short*>(p)[e0 + e] =
+          static_cast<unsigned short>(bf16_bits<SR_PARAM>(f, (e & 1) ? rw[e >> 1] >> 16 : rw[e >> 1] & 0xffffu));
+      t.m[e0 + e] = static_cast<uint8_t>((e < 4 ? x.m.x : x.m.y) >> (8 * (e & 3)));
+      t.r[e0 + e] = static_cast<uint8_t>((e < 4 ? x.r.x : x.r.y) >> (8 * (e & 3)));
     }
-    uint4 rp = make_uint4(0, 0, 0, 0), rs = rp;
-    if (SR_PARAM || SR_STATE) {
-      const unsigned long long at = (t.offset + static_cast<unsigned long long>(e0)) >> 3;
-      const uint2 key = make_uint2(static_cast<uint32_t>(a.seed), static_cast<uint32_t>(a.seed >> 32));
-      const uint32_t c0 = static_cast<uint32_t>(at), c1 = static_cast<uint32_t>(at >> 32);
-      if (SR_PARAM) rp = philox(make_uint4(c0, c1, 0u, 0x3838u), key);
-      if (SR_STATE) rs = philox(make_uint4(c0, c1, 1u, 0x3838u), key);
+    if (lane == i) {
+      m_exp = x.m_exp;
+      r_exp = x.r_exp;
     }
-    mc = encode8<SR_STATE>(mf, rs.x, rs.y);
-    rc = encode8<SR_STATE>(rf, rs.z, rs.w);
-    const uint32_t rw[4] = {rp.x, rp.y, rp.z, rp.w};
-    if (whole) {
-      if (sizeof(P) == 4) {
-        float4* out = reinterpret_cast<float4*>(p + e0);
-        out[0] = make_float4(pf[0], pf[1], pf[2], pf[3]);
-        out[1] = make_float4(pf[4], pf[5], pf[6], pf[7]);
-      } else {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          w[i] = bf16_bits<SR_PARAM>(pf[2 * i], rw[i] & 0xffffu) | bf16_bits<SR_PARAM>(pf[2 * i + 1], rw[i] >> 16) << 16;
-        *reinterpret_cast<uint4*>(p + e0) = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-      *reinterpret_cast<uint2*>(t.m + e0) = mc;
-      *reinterpret_cast<uint2*>(t.r + e0) = rc;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (e0 + e >= t.n) continue;
-        if (sizeof(P) == 4) reinterpret_cast<float*>(p)[e0 + e] = pf[e];
-        else reinterpret_cast<unsigned short*>(p)[e0 + e] =
-            static_cast<unsigned short>(bf16_bits<SR_PARAM>(pf[e], (e & 1) ? rw[e >> 1] >> 16 : rw[e >> 1] & 0xffffu));
-        t.m[e0 + e] = static_cast<uint8_t>((e < 4 ? mc.x : mc.y) >> (8 * (e & 3)));
-        t.r[e0 + e] = static_cast<uint8_t>((e < 4 ? rc.x : rc.y) >> (8 * (e & 3)));
-      }
-    }
-    if (lane == 0) {
-      t.m_exp[b] = static_cast<uint8_t>(m_exp);
-      t.r_exp[b] = static_cast<uint8_t>(r_exp);
-    }
+  }
+  if (lane < mine) {
+    t.m_exp[kept] = static_cast<uint8_t>(m_exp);
+    t.r_exp[kept] = static_cast<uint8_t>(r_exp);
   }
 }
 
 template <class P, class G>
 int launch8(const Table8& tab, const Args8& a, int runs, int sr_param, int sr_state, cudaStream_t s) {
   auto go = [&](auto kern) {
-    kern<<<(runs + A8_WARPS - 1) / A8_WARPS, A8_THREADS, 0, s>>>(tab, a);
+    kern<<<runs, A8_THREADS, 0, s>>>(tab, a);
     return (int)cudaGetLastError();
   };
   if (sizeof(P) == 2 && sr_param)
@@ -244,13 +394,15 @@ int ss_adamw8_many(const long long* tensors, int count, int p_f32, int g_f32, do
     total += (t[6] + A8_BLOCK - 1) / A8_BLOCK;
   }
   Args8 a;
-  a.lr = (float)lr; a.beta1 = (float)beta1; a.beta2 = (float)beta2; a.eps = (float)eps;
+  a.beta1 = (float)beta1; a.beta2 = (float)beta2; a.eps = (float)eps;
   a.c1 = (float)(1.0 - beta1); a.c2 = (float)(1.0 - beta2); a.keep = (float)(1.0 - lr * weight_decay);
-  a.inv_bias1 = (float)(1.0 / (1.0 - pow(beta1, step)));
+  a.minus_lr = (float)(-lr / (1.0 - pow(beta1, step)));
   a.inv_bias2 = (float)(1.0 / sqrt(1.0 - pow(beta2, step)));
   a.grad_scale = (float)grad_scale;
+  a.one = 1.f;
   a.seed = seed ^ (0x9E3779B97F4A7C15ull * (unsigned long long)(step + 1));
-  long long run = total / (148 * 40);
+  // one wave of the three CTAs that fit on an SM, until their runs are long enough to hide their start
+  long long run = (total + 148 * 24 - 1) / (148 * 24);
   run = run < 1 ? 1 : run > 16 ? 16 : run;
   for (int done = 0; done < count;) {
     Table8 tab;
@@ -260,7 +412,7 @@ int ss_adamw8_many(const long long* tensors, int count, int p_f32, int g_f32, do
     for (; done < count && tab.count < A8_TENSORS; ++done) {
       const long long* t = tensors + 8 * done;
       if (t[6] == 0) continue;
-      const long long mine = ((t[6] + A8_BLOCK - 1) / A8_BLOCK + run - 1) / run;
+      const long long mine = ((t[6] + A8_BLOCK - 1) / A8_BLOCK + run * A8_WARPS - 1) / (run * A8_WARPS);
       if (runs + mine > 0x3fffffff) {
         if (tab.count == 0) return -2;
         break;
