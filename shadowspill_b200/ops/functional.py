@@ -527,7 +527,7 @@ def preference_(logits, targets, weights, cu_seqlens, loss_sum, *, beta=0.1, kin
     if logits.stride(1) != 1 or (out is not None and out.stride(1) != 1) or not (targets.is_contiguous() and cu_seqlens.is_contiguous()):
         raise ValueError("logits and their gradient have unit inner stride, targets and cu_seqlens are contiguous")
     with _device_of(logits):
-        work = torch.empty(4 * R + S // 2 + 1, dtype=torch.float32, device=logits.device)
+        work = torch.empty(6 * R + S + 1, dtype=torch.float32, device=logits.device)
         lp = torch.empty(R, dtype=torch.float32, device=logits.device) if logp is None else logp
         _lib.check(_lib.lib().ss_preference(
             logits.data_ptr(), int(logits.dtype == torch.float32), max(logits.stride(0), V), targets.data_ptr(), _ptr(weights),
