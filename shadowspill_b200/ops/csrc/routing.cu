@@ -149,144 +149,290 @@ __device__ __noinline__ int picks_exact(const L* row, const RouteArgs& a, const 
   return mine;
 }
 
-// One warp to a token, expert lane + 32 i in the lane's register i.
-template <int PER, bool LOGITS, class L>
+// PER consecutive values of a row from expert `first` on, -inf behind the last expert.
+template <int PER, class L>
+__device__ __forceinline__ void load_row(const L* row, int first, int E, bool vectors, float (&v)[PER]) {
+  constexpr int BYTES = PER * sizeof(L) < 16 ? PER * sizeof(L) : 16, N = BYTES / sizeof(L);
+  if (vectors && first + PER <= E) {
+#pragma unroll
+    for (int c = 0; c < PER / N; ++c) {
+      alignas(16) L piece[N];
+      if (BYTES == 16) *reinterpret_cast<uint4*>(piece) = *reinterpret_cast<const uint4*>(row + first + c * N);
+      else if (BYTES == 8) *reinterpret_cast<uint2*>(piece) = *reinterpret_cast<const uint2*>(row + first + c * N);
+      else *reinterpret_cast<uint32_t*>(piece) = *reinterpret_cast<const uint32_t*>(row + first + c * N);
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[c * N + i] = load_logit(piece + i);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) v[i] = first + i < E ? load_logit(row + first + i) : -INFINITY;
+}
+
+// LANES to a token, PER consecutive experts to a lane.
+//
+// The k-th largest of the lanes' own maxima bounds the k-th largest key from below: the keys from it on, a dozen where k
+// is 8, are gathered by one place to a lane and sorted. Where they are more than the lanes (one token in twenty for k = 8 of 16
+// lanes; many equal keys), or fewer than k can be compared, the picks are taken one by one instead.
+template <int LANES, int PER, bool LOGITS, class L>
 __global__ void __launch_bounds__(RT_THREADS)
-select_experts_kernel(const L* __restrict__ logits, RouteArgs a, int* __restrict__ ids, float* __restrict__ weights,
+select_experts_kernel(const L* __restrict__ logits, bool vectors, RouteArgs a, int* __restrict__ ids, float* __restrict__ weights,
                       int* __restrict__ counts) {
+  constexpr int TOKENS = 32 / LANES;             // of a warp
   __shared__ int hist[RT_MAX_E];
   __shared__ unsigned char group_of[RT_MAX_E];
+  __shared__ int2 gathered[RT_WARPS][32];
   extern __shared__ double warp_keys[];          // E per warp, where keys may have to be formed in 64 bits
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = lane % LANES, base = lane - rank;
+  const unsigned own = LANES == 32 ? FULL : ((1u << LANES) - 1) << base;         // the lanes of this token
+  const int size = a.E / a.groups, group_lanes = size / PER;
+  const bool lane_groups = size % PER == 0 && (group_lanes & (group_lanes - 1)) == 0;
   for (int e = threadIdx.x; e < a.E; e += RT_THREADS) {
     hist[e] = 0;
-    group_of[e] = static_cast<unsigned char>(e / (a.E / a.groups));
+    if (!LOGITS) group_of[e] = static_cast<unsigned char>(e / size);
   }
   __syncthreads();
-  for (int t = blockIdx.x * RT_WARPS + warp; t < a.T; t += gridDim.x * RT_WARPS) {
-    const L* row = logits + static_cast<long long>(t) * a.ld;
+  double* const keys64 = warp_keys + warp * a.E;
+  const int tokens = gridDim.x * RT_WARPS * TOKENS;
+  for (int t0 = (blockIdx.x * RT_WARPS + warp) * TOKENS; t0 < a.T; t0 += tokens) {
+    const int t = t0 + base / LANES;
+    const bool real = t < a.T;
+    const L* row = logits + static_cast<long long>(real ? t : t0) * a.ld;
+    const int first = rank * PER;
     float v[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) v[i] = lane + 32 * i < a.E ? load_logit(row + lane + 32 * i) : -INFINITY;
+    load_row<PER>(row, first, a.E, vectors, v);
     float top = 0.f, total = 1.f;
     bool bad = false;                            // a softmax with a NaN or +inf in it
     if (!a.sigmoid) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) bad = bad || !(v[i] < INFINITY);
-      bad = __any_sync(FULL, bad);
+      bad = (__ballot_sync(FULL, bad) & own) != 0;
     }
-    if (!a.sigmoid && !(LOGITS && a.renormalize)) {
+    const bool whole = !a.sigmoid && !(LOGITS && a.renormalize);         // the softmax's sum is needed
+    float p[LOGITS ? 1 : PER];                   // exponentials
+    if (whole) {
       top = v[0];
 #pragma unroll
       for (int i = 1; i < PER; ++i) top = fmaxf(top, v[i]);
-      top = row_max(top);
-      float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) sum += v[i] > -INFINITY ? __expf(v[i] - top) : 0.f;
-      total = warp_sum32(sum);
+      for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
+      total = 0.f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const float e = v[i] > -INFINITY ? __expf(v[i] - top) : 0.f;
+        if (!LOGITS) p[i] = e;
+        total += e;
+      }
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) total += __shfl_xor_sync(FULL, total, o);
+      total = fmaxf(total, 1.f);                 // the largest alone is 1; a row of -inf has scores of zero
     }
-    bool again = false;
     float slack = 0.f;
     if (!LOGITS) {
       // errors of a key: the score's (a relative 2^-21 of the largest: exp, its sum, the division) and the sum's rounding
-      slack = a.sigmoid ? 1.5e-6f : 1.5e-6f * __fdividef(1.f, fmaxf(total, 1.f));
-      const float inv = __fdividef(1.f, fmaxf(total, 1.f));
+      const float inv = __fdividef(1.f, total);
+      slack = a.sigmoid ? 1.5e-6f : 1.5e-6f * inv;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const int e = lane + 32 * i;
-        if (a.sigmoid) v[i] = e < a.E ? __fdividef(1.f, 1.f + __expf(-v[i])) : -INFINITY;
-        else if (e < a.E) v[i] = v[i] == -INFINITY ? 0.f : __expf(v[i] - top) * inv;
-        if (e < a.E && a.bias != nullptr) v[i] += a.bias[e];
+        const int e = first + i;
+        if (a.sigmoid) v[i] = __fdividef(1.f, 1.f + __expf(-v[i]));
+        else v[i] = v[i] == v[i] ? p[i] * inv : v[i];
+        if (a.bias != nullptr && e < a.E) v[i] += a.bias[e];
+        if (e >= a.E) v[i] = -INFINITY;
       }
     }
     int key[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) key[i] = lane + 32 * i < a.E ? ordered(v[i]) : INT_MIN;
+    for (int i = 0; i < PER; ++i) key[i] = ordered(v[i]);
+    bool again = false;
     if (!LOGITS && a.groups > 1) {
-      float* keys = reinterpret_cast<float*>(warp_keys + warp * a.E);
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (lane + 32 * i < a.E) keys[lane + 32 * i] = unordered(key[i]);
-      __syncwarp();
-      float gap;
-      const unsigned bits = kept_groups(keys, a, lane, gap);
-      float big = 0.f;                           // group scores are sums of two keys
+      float big = 0.f, gap;                      // group scores are sums of two keys
 #pragma unroll
       for (int i = 0; i < PER; ++i)
         if (key[i] != INT_MIN) big = fmaxf(big, fabsf(v[i]));
-      big = row_max(big);
-      again = a.keep < a.groups && !(gap > 4.f * slack + 5e-7f * big);
-      __syncwarp();
 #pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (lane + 32 * i < a.E && !((bits >> group_of[lane + 32 * i]) & 1)) key[i] = INT_MIN;
-    }
-    int best = INT_MIN, place = 0;
-    auto rescan = [&] {
-      best = key[0];
-      place = 0;
+      for (int o = LANES / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(FULL, big, o));
+      if (lane_groups) {
+        float best = -INFINITY, second = -INFINITY;
 #pragma unroll
-      for (int i = 1; i < PER; ++i)
-        if (key[i] > best) { best = key[i]; place = i; }
-    };
-    rescan();
-    int mine = 0, found = 0;
-    float last = INFINITY;
-    for (; found < a.k && !again; ++found) {
-      const int m = __reduce_max_sync(FULL, best);
-      if (m == INT_MIN) break;
-      const int e = __reduce_min_sync(FULL, best == m ? lane + 32 * place : INT_MAX);
-      if (!LOGITS) {
-        const float f = unordered(m);
-        again = last - f <= 2.f * slack + 2.5e-7f * fabsf(f);
-        last = f;
-      }
-      if (lane == found) mine = e;
-      if ((e & 31) == lane) {
+        for (int i = 0; i < PER; ++i) {
+          const float f = key[i] == INT_MIN ? -INFINITY : v[i];
+          second = fmaxf(second, fminf(best, f));
+          best = fmaxf(best, f);
+        }
+        for (int o = group_lanes >> 1; o > 0; o >>= 1) {
+          const float c = __shfl_xor_sync(FULL, best, o), d = __shfl_xor_sync(FULL, second, o);
+          second = fmaxf(fmaxf(second, d), fminf(best, c));
+          best = fmaxf(best, c);
+        }
+        const float score = size > 1 ? best + second : best;
+        const int group = rank / group_lanes;
+        int ahead = 0;                           // groups that come before this lane's
+        for (int g = 0; g < a.groups; ++g) {
+          const float other = __shfl_sync(FULL, score, base + g * group_lanes);
+          ahead += other > score || (other == score && g < group);
+        }
+        const bool in = group < a.groups, kept = in && ahead < a.keep;
+        float worst = kept ? score : INFINITY, left = in && !kept ? score : -INFINITY;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) {
+          worst = fminf(worst, __shfl_xor_sync(FULL, worst, o));
+          left = fmaxf(left, __shfl_xor_sync(FULL, left, o));
+        }
+        gap = worst - left;
+        if (!kept) {
+#pragma unroll
+          for (int i = 0; i < PER; ++i) key[i] = INT_MIN;
+        }
+      } else {
+        float* keys = reinterpret_cast<float*>(keys64);
+        unsigned bits = 0;
+        gap = 0.f;
+        for (int part = 0; part < TOKENS; ++part) {          // the warp's tokens one after the other
+          if (base == part * LANES) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+              if (first + i < a.E) keys[first + i] = unordered(key[i]);
+          }
+          __syncwarp();
+          float g;
+          const unsigned b = kept_groups(keys, a, lane, g);
+          if (base == part * LANES) { bits = b; gap = g; }
+          __syncwarp();
+        }
 #pragma unroll
         for (int i = 0; i < PER; ++i)
-          if (i == place) key[i] = INT_MIN;
-        rescan();
+          if (first + i < a.E && !((bits >> group_of[first + i]) & 1)) key[i] = INT_MIN;
       }
+      again = a.keep < a.groups && !(gap > 4.f * slack + 5e-7f * big);
+    }
+    // the k-th largest of the lanes' maxima
+    int most = key[0];
+#pragma unroll
+    for (int i = 1; i < PER; ++i) most = max(most, key[i]);
+#pragma unroll
+    for (int n = 2; n <= LANES; n *= 2)
+#pragma unroll
+      for (int o = n / 2; o > 0; o >>= 1) {
+        const int other = __shfl_xor_sync(FULL, most, o);
+        const bool up = (((rank & n) == 0) == ((rank & o) == 0));          // this lane keeps the larger
+        most = up ? max(most, other) : min(most, other);
+      }
+    const int least = __shfl_sync(FULL, most, base + min(a.k, LANES) - 1);
+    int from = least;
+    if (!LOGITS && least != INT_MIN) {           // and what a key's error may put before it
+      const float f = unordered(least);
+      from = ordered(f - (2.f * slack + 2.5e-7f * fabsf(f)));
+    }
+    unsigned chosen = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) chosen |= static_cast<unsigned>(key[i] >= from) << i;
+    int place = __popc(chosen), all;
+    {
+      const int n = place;
+#pragma unroll
+      for (int o = 1; o < LANES; o *= 2) {
+        const int before = __shfl_up_sync(FULL, place, o, LANES);
+        if (rank >= o) place += before;
+      }
+      all = __shfl_sync(FULL, place, base + LANES - 1);
+      place -= n;
+    }
+    const bool sorted = least != INT_MIN && all <= LANES && a.k <= LANES;
+    int mine = 0;
+    if (__any_sync(FULL, sorted)) {
+      if (sorted) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          if ((chosen >> i) & 1) gathered[warp][base + place++] = make_int2(key[i], first + i);
+      }
+      __syncwarp();
+      int2 c = sorted && rank < all ? gathered[warp][lane] : make_int2(INT_MIN, INT_MAX);
+      __syncwarp();
+#pragma unroll
+      for (int n = 2; n <= LANES; n *= 2)
+#pragma unroll
+        for (int o = n / 2; o > 0; o >>= 1) {
+          const int2 other = make_int2(__shfl_xor_sync(FULL, c.x, o), __shfl_xor_sync(FULL, c.y, o));
+          const bool up = (((rank & n) == 0) == ((rank & o) == 0));
+          const bool ahead = other.x > c.x || (other.x == c.x && other.y < c.y);
+          if (ahead == up) c = other;
+        }
+      mine = c.y;
+      if (!LOGITS) {
+        const int next = __shfl_down_sync(FULL, c.x, 1, LANES);
+        const float f = unordered(c.x), g = unordered(next);
+        const bool close = rank < a.k && rank + 1 < all && f - g <= 2.f * slack + 2.5e-7f * fabsf(f);
+        const unsigned near = __ballot_sync(FULL, close && sorted);        // all lanes of the warp take part, whatever `again` is
+        again = again || (near & own) != 0;
+      }
+    }
+    const bool one_by_one = LOGITS && !sorted;
+    if (!LOGITS) again = again || !sorted;
+    if (LOGITS && __any_sync(FULL, one_by_one)) {
+      int last_key = INT_MAX, last_id = -1, left = -1, found = -1;       // the pick before, of those that compare, then of the rest
+      for (int j = 0; j < a.k; ++j) {
+        int best = INT_MIN, at = INT_MAX;        // the largest behind the last pick
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const bool behind = key[i] < last_key || (key[i] == last_key && first + i > last_id);
+          if (behind && key[i] > best) { best = key[i]; at = first + i; }
+        }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) {
+          const int b = __shfl_xor_sync(FULL, best, o), w = __shfl_xor_sync(FULL, at, o);
+          if (b > best || (b == best && w < at)) { best = b; at = w; }
+        }
+        // nothing left that compares: the first experts that do not, in their order (looked for by all lanes: the warp's tokens
+        // differ in this)
+        int rest = INT_MAX;
+#pragma unroll
+        for (int i = PER - 1; i >= 0; --i)
+          if (first + i < a.E && key[i] == INT_MIN && first + i > left) rest = first + i;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) rest = min(rest, __shfl_xor_sync(FULL, rest, o));
+        if (best == INT_MIN) {
+          at = left = rest;
+        } else {
+          last_key = best;
+          last_id = at;
+        }
+        if (rank == j) found = at;
+      }
+      if (one_by_one) mine = found;
     }
     if (!LOGITS) {
-      if (!again && found == a.k) {
-        const int m = __reduce_max_sync(FULL, best);
-        const float f = unordered(m);
-        again = m != INT_MIN && last - f <= 2.f * slack + 2.5e-7f * fabsf(f);
-      }
-      again = again || found < a.k;
-      if (again) mine = picks_exact<PER>(row, a, group_of, warp_keys + warp * a.E, lane);
-    } else if (found < a.k) {                    // fewer than k comparable logits: the first experts not yet picked
-      unsigned taken = 0;
-      for (int j = 0; j < found; ++j) {
-        const int e = __shfl_sync(FULL, mine, j);
-        if ((e & 31) == lane) taken |= 1u << (e >> 5);
-      }
-      for (; found < a.k; ++found) {
-        int left = INT_MAX;
-        for (int i = PER - 1; i >= 0; --i)
-          if (lane + 32 * i < a.E && !((taken >> i) & 1)) left = lane + 32 * i;
-        const int e = __reduce_min_sync(FULL, left);
-        if ((e & 31) == lane) taken |= 1u << (e >> 5);
-        if (lane == found) mine = e;
+      unsigned redo = __ballot_sync(FULL, again && rank == 0 && real);
+      while (redo) {                             // the whole warp, token by token
+        const int at = __ffs(redo) - 1;
+        redo &= redo - 1;
+        const int pick = picks_exact<RT_MAX_E / 32>(logits + static_cast<long long>(t0 + at / LANES) * a.ld, a, group_of, keys64, lane);
+        const int moved = __shfl_sync(FULL, pick, rank);
+        if (base == at) mine = moved;
       }
     }
-    const bool pick = lane < a.k;
+    const bool pick = real && rank < a.k;
     const float x = pick ? load_logit(row + mine) : -INFINITY;
     float s;
     if (a.sigmoid) {
       s = pick ? __fdividef(1.f, 1.f + __expf(-x)) : 0.f;
     } else {
-      if (LOGITS && a.renormalize) top = row_max(x);      // the scores' common factor leaves with the renormalisation
+      if (!whole) {                              // the scores' common factor leaves with the renormalisation
+        top = x > -INFINITY ? x : -INFINITY;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
+      }
       s = !pick || x == -INFINITY ? 0.f : __expf(x - top);
-      if (!(LOGITS && a.renormalize)) s = __fdividef(s, fmaxf(total, 1.f));
+      if (whole) s = __fdividef(s, total);
       if (bad) s = NAN;
     }
-    const float w = a.renormalize ? a.scale * __fdividef(s, warp_sum32(s) + 1e-20f) : a.scale * s;
+    float sum = s;
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL, sum, o);
+    const float w = a.renormalize ? a.scale * __fdividef(s, sum + 1e-20f) : a.scale * s;
     if (pick) {
-      ids[static_cast<long long>(t) * a.k + lane] = mine;
-      weights[static_cast<long long>(t) * a.k + lane] = w;
+      ids[static_cast<long long>(t) * a.k + rank] = mine;
+      weights[static_cast<long long>(t) * a.k + rank] = w;
       atomicAdd(&hist[mine], 1);
     }
   }
@@ -366,29 +512,36 @@ int ss_select_experts(const void* logits, int bf16_logits, long long ld, const f
   const RouteArgs a{T, E, k, groups, keep_groups, sigmoid, renormalize, ld, scale, bias};
   if (!fits(a)) return -2;
   cudaStream_t s = (cudaStream_t)stream;
-  const int blocks = (T + RT_WARPS - 1) / RT_WARPS, grid = blocks < 1 ? 1 : blocks < 148 * 8 ? blocks : 148 * 8;
+  // Half a warp to a token where it has twice as many lanes as picks, with up to 16 experts to a lane.
+  const bool halves = 2 * k <= 16 && E <= 256;
+  const int lanes = halves ? 16 : 32, per_block = RT_WARPS * (halves ? 2 : 1);
+  const int blocks = (T + per_block - 1) / per_block, grid = blocks < 1 ? 1 : blocks < 148 * 8 ? blocks : 148 * 8;
   if (grid > 1) {                                // a single block writes the counts whole
     const cudaError_t e = cudaMemsetAsync(counts, 0, sizeof(int) * E, s);
     if (e != cudaSuccess) return (int)e;
   }
   const bool plain = bias == nullptr && groups == 1;
   auto go = [&](auto kern, auto* x) {
-    kern<<<grid, RT_THREADS, plain ? 0 : sizeof(double) * E * RT_WARPS, s>>>(x, a, ids, weights, counts);
+    const bool vectors = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld * sizeof(*x) % 16 == 0;
+    kern<<<grid, RT_THREADS, plain ? 0 : sizeof(double) * E * RT_WARPS, s>>>(x, vectors, a, ids, weights, counts);
     return (int)cudaGetLastError();
   };
-  auto by_type = [&](auto* x) {
-    using L = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
-    if (plain) {
-      if (E <= 64) return go(select_experts_kernel<2, true, L>, x);
-      if (E <= 128) return go(select_experts_kernel<4, true, L>, x);
-      if (E <= 256) return go(select_experts_kernel<8, true, L>, x);
-      return go(select_experts_kernel<16, true, L>, x);
+  auto by_mode = [&](auto* x, auto logits_only) {
+    using X = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
+    constexpr bool P = decltype(logits_only)::value;
+    const int per = (E + lanes - 1) / lanes;
+    if (halves) {
+      if (per <= 2) return go(select_experts_kernel<16, 2, P, X>, x);
+      if (per <= 4) return go(select_experts_kernel<16, 4, P, X>, x);
+      if (per <= 8) return go(select_experts_kernel<16, 8, P, X>, x);
+      return go(select_experts_kernel<16, 16, P, X>, x);
     }
-    if (E <= 64) return go(select_experts_kernel<2, false, L>, x);
-    if (E <= 128) return go(select_experts_kernel<4, false, L>, x);
-    if (E <= 256) return go(select_experts_kernel<8, false, L>, x);
-    return go(select_experts_kernel<16, false, L>, x);
+    if (per <= 2) return go(select_experts_kernel<32, 2, P, X>, x);
+    if (per <= 4) return go(select_experts_kernel<32, 4, P, X>, x);
+    if (per <= 8) return go(select_experts_kernel<32, 8, P, X>, x);
+    return go(select_experts_kernel<32, 16, P, X>, x);
   };
+  auto by_type = [&](auto* x) { return plain ? by_mode(x, std::true_type()) : by_mode(x, std::false_type()); };
   return bf16_logits ? by_type((const __nv_bfloat16*)logits) : by_type((const float*)logits);
 }
 
