@@ -33,15 +33,23 @@ __device__ __forceinline__ float warp_sum32(float v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
   return v;
 }
-// Signed integers in the order of the floats; -inf and NaN compare lowest and equal.
-__device__ __forceinline__ int ordered(float v) {
-  const int b = __float_as_int(v + 0.f);         // -0 and 0 are equal
-  return v > -INFINITY ? b ^ ((b >> 31) & 0x7fffffff) : INT_MIN;
+__device__ __forceinline__ float warp_max32(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, o));
+  return v;
 }
-__device__ __forceinline__ float unordered(int o) {
-  return o == INT_MIN ? -INFINITY : __int_as_float(o ^ ((o >> 31) & 0x7fffffff));
+
+// exp and 1 / (1 + exp(-x)) without the steps that keep denormal results.
+__device__ __forceinline__ float exp_of(float x) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * 1.44269504f));
+  return e;
 }
-__device__ __forceinline__ float row_max(float v) { return unordered(__reduce_max_sync(FULL, ordered(v))); }
+__device__ __forceinline__ float sigmoid_of(float x) {
+  float s;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + exp_of(-x)));
+  return s;
+}
 
 struct RouteArgs {
   int T, E, k, groups, keep, sigmoid, renormalize;
@@ -101,7 +109,7 @@ template <int PER, class L>
 __device__ __noinline__ int picks_exact(const L* row, const RouteArgs& a, const unsigned char* group_of, double* keys, int lane) {
   float top = -INFINITY;
   for (int e = lane; e < a.E; e += 32) top = fmaxf(top, load_logit(row + e));
-  top = row_max(top);
+  top = warp_max32(top);
   double total = 0.0;
   if (!a.sigmoid) {
     for (int e = lane; e < a.E; e += 32) {
@@ -174,14 +182,15 @@ __device__ __forceinline__ void load_row(const L* row, int first, int E, bool ve
 // The k-th largest of the lanes' own maxima bounds the k-th largest key from below: the keys from it on, a dozen where k
 // is 8, are gathered by one place to a lane and sorted. Where they are more than the lanes (one token in twenty for k = 8 of 16
 // lanes; many equal keys), or fewer than k can be compared, the picks are taken one by one instead.
+constexpr int rt_resident(int per) { return per == 16 ? 7 : 8; }     // blocks that an SM's registers hold
 template <int LANES, int PER, bool LOGITS, class L>
-__global__ void __launch_bounds__(RT_THREADS)
-select_experts_kernel(const L* __restrict__ logits, bool vectors, RouteArgs a, int* __restrict__ ids, float* __restrict__ weights,
+__global__ void __launch_bounds__(RT_THREADS, rt_resident(PER))
+select_experts_kernel(const L* __restrict__ logits, bool vectors, bool bias_vectors, RouteArgs a, int* __restrict__ ids, float* __restrict__ weights,
                       int* __restrict__ counts) {
   constexpr int TOKENS = 32 / LANES;             // of a warp
   __shared__ int hist[RT_MAX_E];
   __shared__ unsigned char group_of[RT_MAX_E];
-  __shared__ int2 gathered[RT_WARPS][32];
+  __shared__ float2 gathered[RT_WARPS][32];
   extern __shared__ double warp_keys[];          // E per warp, where keys may have to be formed in 64 bits
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = lane % LANES, base = lane - rank;
   const unsigned own = LANES == 32 ? FULL : ((1u << LANES) - 1) << base;         // the lanes of this token
@@ -209,7 +218,6 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, RouteArgs a, i
       bad = (__ballot_sync(FULL, bad) & own) != 0;
     }
     const bool whole = !a.sigmoid && !(LOGITS && a.renormalize);         // the softmax's sum is needed
-    float p[LOGITS ? 1 : PER];                   // exponentials
     if (whole) {
       top = v[0];
 #pragma unroll
@@ -217,48 +225,43 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, RouteArgs a, i
 #pragma unroll
       for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
       total = 0.f;
+      const float none = top == -INFINITY ? 0.f : top;       // a row of -inf: exponentials of zero
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const float e = v[i] > -INFINITY ? __expf(v[i] - top) : 0.f;
-        if (!LOGITS) p[i] = e;
+        const float e = exp_of(v[i] - none);
+        if (!LOGITS) v[i] = e;
         total += e;
       }
 #pragma unroll
       for (int o = LANES / 2; o > 0; o >>= 1) total += __shfl_xor_sync(FULL, total, o);
-      total = fmaxf(total, 1.f);                 // the largest alone is 1; a row of -inf has scores of zero
+      total = fmaxf(total, 1.f);                 // the largest alone is 1
     }
+    // v becomes the keys: -inf for what cannot be picked or compared
     float slack = 0.f;
     if (!LOGITS) {
       // errors of a key: the score's (a relative 2^-21 of the largest: exp, its sum, the division) and the sum's rounding
       const float inv = __fdividef(1.f, total);
       slack = a.sigmoid ? 1.5e-6f : 1.5e-6f * inv;
+      float b[PER];
+      if (a.bias != nullptr) load_row<PER>(a.bias, first, a.E, bias_vectors, b);
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const int e = first + i;
-        if (a.sigmoid) v[i] = __fdividef(1.f, 1.f + __expf(-v[i]));
-        else v[i] = v[i] == v[i] ? p[i] * inv : v[i];
-        if (a.bias != nullptr && e < a.E) v[i] += a.bias[e];
-        if (e >= a.E) v[i] = -INFINITY;
+        v[i] = a.sigmoid ? sigmoid_of(v[i]) : v[i] * inv;
+        if (a.bias != nullptr) v[i] += b[i];     // -inf behind the last expert
+        else if (first + i >= a.E) v[i] = -INFINITY;
       }
     }
-    int key[PER];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) key[i] = ordered(v[i]);
+    for (int i = 0; i < PER; ++i) v[i] = fmaxf(v[i], -INFINITY);         // NaN
     bool again = false;
     if (!LOGITS && a.groups > 1) {
-      float big = 0.f, gap;                      // group scores are sums of two keys
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (key[i] != INT_MIN) big = fmaxf(big, fabsf(v[i]));
-#pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(FULL, big, o));
+      float gap, big;                            // big: the largest of the keys that group scores are sums of
       if (lane_groups) {
         float best = -INFINITY, second = -INFINITY;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-          const float f = key[i] == INT_MIN ? -INFINITY : v[i];
-          second = fmaxf(second, fminf(best, f));
-          best = fmaxf(best, f);
+          second = fmaxf(second, fminf(best, v[i]));
+          best = fmaxf(best, v[i]);
         }
         for (int o = group_lanes >> 1; o > 0; o >>= 1) {
           const float c = __shfl_xor_sync(FULL, best, o), d = __shfl_xor_sync(FULL, second, o);
@@ -274,25 +277,31 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, RouteArgs a, i
         }
         const bool in = group < a.groups, kept = in && ahead < a.keep;
         float worst = kept ? score : INFINITY, left = in && !kept ? score : -INFINITY;
+        big = fmaxf(best > -INFINITY ? fabsf(best) : 0.f, second > -INFINITY ? fabsf(second) : 0.f);
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) {
           worst = fminf(worst, __shfl_xor_sync(FULL, worst, o));
           left = fmaxf(left, __shfl_xor_sync(FULL, left, o));
+          big = fmaxf(big, __shfl_xor_sync(FULL, big, o));
         }
         gap = worst - left;
         if (!kept) {
 #pragma unroll
-          for (int i = 0; i < PER; ++i) key[i] = INT_MIN;
+          for (int i = 0; i < PER; ++i) v[i] = -INFINITY;
         }
       } else {
         float* keys = reinterpret_cast<float*>(keys64);
         unsigned bits = 0;
-        gap = 0.f;
+        gap = big = 0.f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) big = fmaxf(big, v[i] > -INFINITY ? fabsf(v[i]) : 0.f);
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(FULL, big, o));
         for (int part = 0; part < TOKENS; ++part) {          // the warp's tokens one after the other
           if (base == part * LANES) {
 #pragma unroll
             for (int i = 0; i < PER; ++i)
-              if (first + i < a.E) keys[first + i] = unordered(key[i]);
+              if (first + i < a.E) keys[first + i] = v[i];
           }
           __syncwarp();
           float g;
@@ -302,31 +311,27 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, RouteArgs a, i
         }
 #pragma unroll
         for (int i = 0; i < PER; ++i)
-          if (first + i < a.E && !((bits >> group_of[first + i]) & 1)) key[i] = INT_MIN;
+          if (first + i < a.E && !((bits >> group_of[first + i]) & 1)) v[i] = -INFINITY;
       }
       again = a.keep < a.groups && !(gap > 4.f * slack + 5e-7f * big);
     }
     // the k-th largest of the lanes' maxima
-    int most = key[0];
+    float most = v[0];
 #pragma unroll
-    for (int i = 1; i < PER; ++i) most = max(most, key[i]);
+    for (int i = 1; i < PER; ++i) most = fmaxf(most, v[i]);
 #pragma unroll
     for (int n = 2; n <= LANES; n *= 2)
 #pragma unroll
       for (int o = n / 2; o > 0; o >>= 1) {
-        const int other = __shfl_xor_sync(FULL, most, o);
+        const float other = __shfl_xor_sync(FULL, most, o);
         const bool up = (((rank & n) == 0) == ((rank & o) == 0));          // this lane keeps the larger
-        most = up ? max(most, other) : min(most, other);
+        most = up ? fmaxf(most, other) : fminf(most, other);
       }
-    const int least = __shfl_sync(FULL, most, base + min(a.k, LANES) - 1);
-    int from = least;
-    if (!LOGITS && least != INT_MIN) {           // and what a key's error may put before it
-      const float f = unordered(least);
-      from = ordered(f - (2.f * slack + 2.5e-7f * fabsf(f)));
-    }
+    const float least = __shfl_sync(FULL, most, base + min(a.k, LANES) - 1);
+    const float from = LOGITS ? least : least - (2.f * slack + 2.5e-7f * fabsf(least));      // and what an error may put before it
     unsigned chosen = 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) chosen |= static_cast<unsigned>(key[i] >= from) << i;
+    for (int i = 0; i < PER; ++i) chosen |= static_cast<unsigned>(v[i] >= from) << i;
     int place = __popc(chosen), all;
     {
       const int n = place;
@@ -338,31 +343,37 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, RouteArgs a, i
       all = __shfl_sync(FULL, place, base + LANES - 1);
       place -= n;
     }
-    const bool sorted = least != INT_MIN && all <= LANES && a.k <= LANES;
+    const bool sorted = least > -INFINITY && all <= LANES && a.k <= LANES;
     int mine = 0;
     if (__any_sync(FULL, sorted)) {
       if (sorted) {
 #pragma unroll
         for (int i = 0; i < PER; ++i)
-          if ((chosen >> i) & 1) gathered[warp][base + place++] = make_int2(key[i], first + i);
+          if ((chosen >> i) & 1) gathered[warp][base + place++] = make_float2(v[i], __int_as_float(first + i));
       }
       __syncwarp();
-      int2 c = sorted && rank < all ? gathered[warp][lane] : make_int2(INT_MIN, INT_MAX);
+      float key = -INFINITY;
+      int id = INT_MAX;
+      if (sorted && rank < all) {
+        const float2 c = gathered[warp][lane];
+        key = c.x;
+        id = __float_as_int(c.y);
+      }
       __syncwarp();
 #pragma unroll
       for (int n = 2; n <= LANES; n *= 2)
 #pragma unroll
         for (int o = n / 2; o > 0; o >>= 1) {
-          const int2 other = make_int2(__shfl_xor_sync(FULL, c.x, o), __shfl_xor_sync(FULL, c.y, o));
+          const float other = __shfl_xor_sync(FULL, key, o);
+          const int whose = __shfl_xor_sync(FULL, id, o);
           const bool up = (((rank & n) == 0) == ((rank & o) == 0));
-          const bool ahead = other.x > c.x || (other.x == c.x && other.y < c.y);
-          if (ahead == up) c = other;
+          const bool ahead = other > key || (other == key && whose < id);
+          if (ahead == up) { key = other; id = whose; }
         }
-      mine = c.y;
+      mine = id;
       if (!LOGITS) {
-        const int next = __shfl_down_sync(FULL, c.x, 1, LANES);
-        const float f = unordered(c.x), g = unordered(next);
-        const bool close = rank < a.k && rank + 1 < all && f - g <= 2.f * slack + 2.5e-7f * fabsf(f);
+        const float next = __shfl_down_sync(FULL, key, 1, LANES);
+        const bool close = rank < a.k && rank + 1 < all && key - next <= 2.f * slack + 2.5e-7f * fabsf(key);
         const unsigned near = __ballot_sync(FULL, close && sorted);        // all lanes of the warp take part, whatever `again` is
         again = again || (near & own) != 0;
       }
@@ -370,17 +381,20 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, RouteArgs a, i
     const bool one_by_one = LOGITS && !sorted;
     if (!LOGITS) again = again || !sorted;
     if (LOGITS && __any_sync(FULL, one_by_one)) {
-      int last_key = INT_MAX, last_id = -1, left = -1, found = -1;       // the pick before, of those that compare, then of the rest
+      float last_key = INFINITY;                 // the pick before, of those that compare, then of the rest
+      int last_id = -1, left = -1, found = -1;
       for (int j = 0; j < a.k; ++j) {
-        int best = INT_MIN, at = INT_MAX;        // the largest behind the last pick
+        float best = -INFINITY;                  // the largest behind the last pick
+        int at = INT_MAX;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-          const bool behind = key[i] < last_key || (key[i] == last_key && first + i > last_id);
-          if (behind && key[i] > best) { best = key[i]; at = first + i; }
+          const bool behind = v[i] < last_key || (v[i] == last_key && first + i > last_id);
+          if (behind && v[i] > best) { best = v[i]; at = first + i; }
         }
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) {
-          const int b = __shfl_xor_sync(FULL, best, o), w = __shfl_xor_sync(FULL, at, o);
+          const float b = __shfl_xor_sync(FULL, best, o);
+          const int w = __shfl_xor_sync(FULL, at, o);
           if (b > best || (b == best && w < at)) { best = b; at = w; }
         }
         // nothing left that compares: the first experts that do not, in their order (looked for by all lanes: the warp's tokens
@@ -388,10 +402,10 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, RouteArgs a, i
         int rest = INT_MAX;
 #pragma unroll
         for (int i = PER - 1; i >= 0; --i)
-          if (first + i < a.E && key[i] == INT_MIN && first + i > left) rest = first + i;
+          if (first + i < a.E && v[i] == -INFINITY && first + i > left) rest = first + i;
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) rest = min(rest, __shfl_xor_sync(FULL, rest, o));
-        if (best == INT_MIN) {
+        if (best == -INFINITY) {
           at = left = rest;
         } else {
           last_key = best;
@@ -415,14 +429,14 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, RouteArgs a, i
     const float x = pick ? load_logit(row + mine) : -INFINITY;
     float s;
     if (a.sigmoid) {
-      s = pick ? __fdividef(1.f, 1.f + __expf(-x)) : 0.f;
+      s = pick ? sigmoid_of(x) : 0.f;
     } else {
       if (!whole) {                              // the scores' common factor leaves with the renormalisation
         top = x > -INFINITY ? x : -INFINITY;
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
       }
-      s = !pick || x == -INFINITY ? 0.f : __expf(x - top);
+      s = !pick || x == -INFINITY ? 0.f : exp_of(x - top);
       if (whole) s = __fdividef(s, total);
       if (bad) s = NAN;
     }
@@ -463,18 +477,18 @@ select_experts_bwd_kernel(const L* __restrict__ logits, RouteArgs a, const int* 
     if (whole) {
       top = -INFINITY;
       for (int e = lane; e < a.E; e += 32) top = fmaxf(top, load_logit(row + e));
-      top = row_max(top);
+      top = warp_max32(top);
       float sum = 0.f;
       for (int e = lane; e < a.E; e += 32) {
         const float y = load_logit(row + e);
-        sum += y == -INFINITY ? 0.f : __expf(y - top);
+        sum += y == -INFINITY ? 0.f : exp_of(y - top);
       }
       total = warp_sum32(sum);
     } else if (!a.sigmoid) {
-      top = row_max(x);
+      top = warp_max32(x);
     }
-    if (a.sigmoid) s = in ? __fdividef(1.f, 1.f + __expf(-x)) : 0.f;
-    else s = x == -INFINITY ? 0.f : __fdividef(__expf(x - top), fmaxf(total, 1.f));
+    if (a.sigmoid) s = in ? sigmoid_of(x) : 0.f;
+    else s = x == -INFINITY ? 0.f : __fdividef(exp_of(x - top), fmaxf(total, 1.f));
     float d = a.scale * dw;
     if (a.renormalize) {
       const float inv = __fdividef(1.f, warp_sum32(s) + 1e-20f);
@@ -484,13 +498,13 @@ select_experts_bwd_kernel(const L* __restrict__ logits, RouteArgs a, const int* 
       inner = warp_sum32(d * s);
       for (int e = lane; e < a.E; e += 32) {
         const float y = load_logit(row + e);
-        store_logit(out + e, y == -INFINITY ? 0.f : -__fdividef(__expf(y - top), fmaxf(total, 1.f)) * inner);
+        store_logit(out + e, y == -INFINITY ? 0.f : -__fdividef(exp_of(y - top), fmaxf(total, 1.f)) * inner);
       }
     } else {
       for (int e = lane; e < a.E; e += 32) store_logit(out + e, 0.f);
     }
     __syncwarp();                                // the picks overwrite what another lane wrote above
-    if (in) store_logit(out + id, a.sigmoid ? d * s * __fdividef(1.f, 1.f + __expf(x)) : s * (d - inner));
+    if (in) store_logit(out + id, a.sigmoid ? d * s * sigmoid_of(-x) : s * (d - inner));
   }
 }
 
@@ -515,7 +529,8 @@ int ss_select_experts(const void* logits, int bf16_logits, long long ld, const f
   // Half a warp to a token where it has twice as many lanes as picks, with up to 16 experts to a lane.
   const bool halves = 2 * k <= 16 && E <= 256;
   const int lanes = halves ? 16 : 32, per_block = RT_WARPS * (halves ? 2 : 1);
-  const int blocks = (T + per_block - 1) / per_block, grid = blocks < 1 ? 1 : blocks < 148 * 8 ? blocks : 148 * 8;
+  const int per = (E + lanes - 1) / lanes, most = 148 * rt_resident(per <= 8 ? 8 : 16);
+  const int blocks = (T + per_block - 1) / per_block, grid = blocks < 1 ? 1 : blocks < most ? blocks : most;
   if (grid > 1) {                                // a single block writes the counts whole
     const cudaError_t e = cudaMemsetAsync(counts, 0, sizeof(int) * E, s);
     if (e != cudaSuccess) return (int)e;
@@ -523,13 +538,12 @@ int ss_select_experts(const void* logits, int bf16_logits, long long ld, const f
   const bool plain = bias == nullptr && groups == 1;
   auto go = [&](auto kern, auto* x) {
     const bool vectors = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld * sizeof(*x) % 16 == 0;
-    kern<<<grid, RT_THREADS, plain ? 0 : sizeof(double) * E * RT_WARPS, s>>>(x, vectors, a, ids, weights, counts);
+    kern<<<grid, RT_THREADS, plain ? 0 : sizeof(double) * E * RT_WARPS, s>>>(x, vectors, reinterpret_cast<uintptr_t>(bias) % 16 == 0, a, ids, weights, counts);
     return (int)cudaGetLastError();
   };
   auto by_mode = [&](auto* x, auto logits_only) {
     using X = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
     constexpr bool P = decltype(logits_only)::value;
-    const int per = (E + lanes - 1) / lanes;
     if (halves) {
       if (per <= 2) return go(select_experts_kernel<16, 2, P, X>, x);
       if (per <= 4) return go(select_experts_kernel<16, 4, P, X>, x);
