@@ -18,8 +18,8 @@ _LIB_PATH = Path(__file__).resolve().parent / "libss_kernels.so"
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
-c_int, c_ll, c_ull, c_f, c_d, c_p = (ctypes.c_int, ctypes.c_longlong, ctypes.c_ulonglong, ctypes.c_float,
-                                     ctypes.c_double, ctypes.c_void_p)
+c_int, c_ll, c_ull, c_f, c_p = (ctypes.c_int, ctypes.c_longlong, ctypes.c_ulonglong,
+                                ctypes.c_float, ctypes.c_void_p)
 
 _SIGNATURES = {
     "ss_gemm_bf16": [c_p, c_p, c_p, c_int, c_int, c_int, c_ll, c_ll, c_ll, c_int, c_int, c_int,
@@ -47,7 +47,7 @@ _SIGNATURES = {
                     c_ull, c_int, c_int, c_p],
     "ss_adamw_sr_many": [c_p, c_int, c_f, c_f, c_f, c_f, c_f, c_int, c_f, c_ull, c_int, c_int, c_p],
     "ss_adamw_f32": [c_p, c_p, c_p, c_p, c_ll, c_f, c_f, c_f, c_f, c_f, c_int, c_f, c_p],
-    "ss_adamw8_many": [c_p, c_int, c_int, c_int, c_d, c_d, c_d, c_d, c_d, c_int, c_d, c_ull, c_int, c_int, c_p],
+    "ss_adamw8_many": [c_p, c_int, c_int, c_int, c_p, c_int, c_ll, c_int, c_int, c_p],
     "ss_preference": [c_p, c_int, c_ll, c_p, c_p, c_p, c_int, c_int, c_int, c_p, c_f, c_int, c_f, c_int, c_f, c_p, c_p, c_p,
                       c_p, c_ll, c_p, c_p],
     "ss_sumsq": [c_p, c_ll, c_p, c_p, c_int, c_p],

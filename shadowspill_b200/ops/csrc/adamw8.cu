@@ -16,6 +16,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include "launchers.h"
+
 namespace ss {
 namespace {
 
@@ -381,11 +383,12 @@ int launch8(const Table8& tab, const Args8& a, int runs, int sr_param, int sr_st
 extern "C" {
 using namespace ss;
 
-// `tensors`: eight values per tensor, {p, g, m, r, m_exp, r_exp, elements, offset}, in host memory, read before the call
-// returns; no element is in two of them. All parameters are of one type, and all gradients.
-int ss_adamw8_many(const long long* tensors, int count, int p_f32, int g_f32, double lr, double beta1, double beta2, double eps,
-                   double weight_decay, int step, double grad_scale, unsigned long long seed, int sr_param, int sr_state,
-                   void* stream) {
+// `tensors`: eight values per tensor, {p, g, m, r, m_exp, r_exp, elements, offset}, and `hyper`, {lr, beta1, beta2, eps, weight decay,
+// gradient scale}, in host memory, read before the call returns. No element is in two tensors; all parameters are of
+// one type, and all gradients.
+int ss_adamw8_many(const long long* tensors, int count, int p_f32, int g_f32, const double* hyper, int step, long long seed,
+                   int sr_param, int sr_state, void* stream) {
+  const double lr = hyper[0], beta1 = hyper[1], beta2 = hyper[2], eps = hyper[3], weight_decay = hyper[4], grad_scale = hyper[5];
   if (step < 1) return -2;
   long long total = 0;
   for (int i = 0; i < count; ++i) {
@@ -400,7 +403,7 @@ int ss_adamw8_many(const long long* tensors, int count, int p_f32, int g_f32, do
   a.inv_bias2 = (float)(1.0 / sqrt(1.0 - pow(beta2, step)));
   a.grad_scale = (float)grad_scale;
   a.one = 1.f;
-  a.seed = seed ^ (0x9E3779B97F4A7C15ull * (unsigned long long)(step + 1));
+  a.seed = static_cast<unsigned long long>(seed) ^ (0x9E3779B97F4A7C15ull * (unsigned long long)(step + 1));
   // one wave of the three CTAs that fit on an SM, until their runs are long enough to hide their start
   long long run = (total + 148 * 24 - 1) / (148 * 24);
   run = run < 1 ? 1 : run > 16 ? 16 : run;

@@ -1,4 +1,4 @@
-// The hot entry points of ops/functional.py and ops/attention.py in native code: from tensors to the C launchers of
+// The hot entry points of ops/functional.py, ops/attention.py and ops/routing.py in native code: from tensors to the C launchers of
 // libss_kernels.so without a Python statement in between. A launch costs about 2.5 us there; reading its operands'
 // pointers, sizes and strides, allocating the result and converting a dozen arguments in Python took 6 to 9 us more,
 // which bounds models whose kernels are shorter than that.
@@ -13,7 +13,10 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+#include <climits>
 #include <cmath>
+#include <vector>
 
 #include "launchers.h"
 
@@ -35,10 +38,12 @@ at::Tensor empty(at::IntArrayRef sizes, const at::TensorOptions& options) {
 }
 
 // Kernels enqueued by each launcher's successful calls, which _lib adds to those it counts itself.
-enum Entry { GEMM, GEMM2, RESIDUAL, SWIGLU, SWIGLU_BWD, NORM_FWD, NORM_BWD, ROPE, ATTN_FWD, ATTN_BWD, ENTRIES };
+enum Entry { GEMM, GEMM2, RESIDUAL, SWIGLU, SWIGLU_BWD, NORM_FWD, NORM_BWD, ROPE, ATTN_FWD, ATTN_BWD, SELECT, SELECT_BWD, PREFERENCE,
+             PREFERENCE_GRAD, ADAMW8, ENTRIES };
 const char* const kNames[ENTRIES] = {"ss_gemm_bf16", "ss_gemm2_bf16", "ss_gemm2_residual_bf16", "ss_gemm2_swiglu_bf16",
                                      "ss_gemm2_swiglu_bwd_bf16", "ss_rmsnorm_fwd", "ss_rmsnorm_bwd", "ss_rope",
-                                     "ss_attn_fwd", "ss_attn_bwd"};
+                                     "ss_attn_fwd", "ss_attn_bwd", "ss_select_experts", "ss_select_experts_bwd", "ss_preference",
+                                     "ss_preference with its gradient", "ss_adamw8_many"};
 long long g_launched[ENTRIES];           // under the GIL
 
 struct Failed { const char* what; int rc; };
@@ -51,7 +56,8 @@ void launch(Entry e, F* entry, A... args) {
     rc = entry(args...);
   }
   if (rc) throw Failed{kNames[e], rc};
-  g_launched[e] += e == ATTN_BWD ? 3 : 1;        // delta, dQ, dK and dV (as _lib counts them)
+  // delta, dQ, dK and dV; rows and gradient (as _lib counts them)
+  g_launched[e] += e == ATTN_BWD ? 3 : e == PREFERENCE_GRAD ? 2 : 1;
 }
 
 const at::Tensor& tensor(PyObject* o) {
@@ -326,6 +332,156 @@ PyObject* attention_bwd(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
+// A call without a status word: where its kernels go.
+void* stream_of(const at::Tensor& t) {
+  want(t.is_cuda());
+  const auto s = c10::cuda::getCurrentCUDAStream();
+  want(s.device_index() == t.get_device());
+  return s.stream();
+}
+bool on(const at::Tensor& t, const at::Tensor& with) { return t.is_cuda() && t.get_device() == with.get_device(); }
+// 2-D rows of bf16 or fp32 logits; is it fp32?
+bool logits_rows(const at::Tensor& t) {
+  const bool f32 = t.scalar_type() == at::kFloat;
+  want(t.is_cuda() && (f32 || t.scalar_type() == at::kBFloat16) && t.dim() == 2 && t.stride(1) == 1 &&
+       (t.size(0) <= 1 || t.stride(0) >= t.size(1)) && t.size(0) <= INT_MAX && t.size(1) <= INT_MAX);
+  return f32;
+}
+int64_t pitch(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : std::max(t.stride(0), t.size(1)); }
+// A contiguous fp32 vector of n, or none
+float* floats(PyObject* o, int64_t n, const at::Tensor& with) {
+  if (none(o)) return nullptr;
+  const at::Tensor& t = tensor(o);
+  want(on(t, with) && t.scalar_type() == at::kFloat && t.dim() == 1 && t.size(0) == n && t.is_contiguous());
+  return static_cast<float*>(t.data_ptr());
+}
+
+// select_experts(logits, k, sigmoid, bias or None, groups, keep_groups, renormalize, scale) -> (ids, weights, counts)
+PyObject* select_experts(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 8, [&]() -> PyObject* {
+    const at::Tensor& x = tensor(v[0]);
+    const bool f32 = logits_rows(x);
+    void* stream = stream_of(x);
+    const int64_t T = x.size(0), E = x.size(1), k = integer(v[1]), sigmoid = integer(v[2]), groups = integer(v[4]), keep = integer(v[5]);
+    want((sigmoid == 0 || sigmoid == 1) && E >= 1 && E <= 512 && k >= 1 && k <= 32 && groups >= 1 && groups <= 32 && E % groups == 0 &&
+         keep >= 1 && keep <= groups && k <= keep * (E / groups));
+    const float* bias = floats(v[3], E, x);
+    const auto options = x.options().requires_grad(false);
+    at::Tensor ids = empty({T, k}, options.dtype(at::kInt)), weights = empty({T, k}, options.dtype(at::kFloat)),
+               counts = empty({E}, options.dtype(at::kInt));
+    launch(SELECT, ss_select_experts, x.data_ptr(), !f32, pitch(x), bias, T, E, k, groups, keep, sigmoid, v[6] == Py_True,
+           static_cast<float>(number(v[7])), static_cast<int*>(ids.data_ptr()), static_cast<float*>(weights.data_ptr()),
+           static_cast<int*>(counts.data_ptr()), stream);
+    return Py_BuildValue("(NNN)", wrap(std::move(ids)), wrap(std::move(weights)), wrap(std::move(counts)));
+  });
+}
+
+// select_experts_bwd(logits, ids, dweights, sigmoid, renormalize, scale) -> dlogits
+PyObject* select_experts_bwd(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 6, [&]() -> PyObject* {
+    const at::Tensor &x = tensor(v[0]), &ids = tensor(v[1]), &dw = tensor(v[2]);
+    const bool f32 = logits_rows(x);
+    void* stream = stream_of(x);
+    contiguous(ids, at::kInt);
+    contiguous(dw, at::kFloat);
+    want(ids.dim() == 2 && dw.sizes() == ids.sizes() && ids.size(0) == x.size(0) && on(ids, x) && on(dw, x));
+    const int64_t T = x.size(0), E = x.size(1), k = ids.size(1), sigmoid = integer(v[3]);
+    want((sigmoid == 0 || sigmoid == 1) && E >= 1 && E <= 512 && k >= 1 && k <= 32 && k <= E);
+    at::Tensor out = empty({T, E}, x.options().requires_grad(false));
+    launch(SELECT_BWD, ss_select_experts_bwd, x.data_ptr(), !f32, pitch(x), static_cast<const int*>(ids.data_ptr()),
+           static_cast<const float*>(dw.data_ptr()), T, E, k, sigmoid, v[4] == Py_True, static_cast<float>(number(v[5])),
+           out.data_ptr(), stream);
+    return wrap(std::move(out));
+  });
+}
+
+// preference(logits, targets, weights or None, cu_seqlens, loss_sum, beta, kind, smoothing, average, ref_logp or None, grad_scale,
+//            write_grad, grad or None, sums or None, logp or None) -> loss_sum
+PyObject* preference(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 15, [&]() -> PyObject* {
+    const at::Tensor &x = tensor(v[0]), &targets = tensor(v[1]), &cu = tensor(v[3]);
+    const bool f32 = logits_rows(x);
+    void* stream = stream_of(x);
+    const int64_t R = x.size(0), V = x.size(1);
+    contiguous(targets, at::kLong);
+    contiguous(cu, at::kInt);
+    const int64_t S = cu.numel() - 1;
+    want(targets.dim() == 1 && targets.size(0) == R && on(targets, x) && cu.dim() == 1 && on(cu, x) && S >= 0 && S % 2 == 0 && V >= 1);
+    const double beta = number(v[5]), smoothing = number(v[7]);
+    const long long kind = integer(v[6]);
+    want(beta > 0 && smoothing >= 0 && smoothing < 1 && kind >= 0 && kind <= 2 && (kind == 0 || smoothing == 0));
+    const float* weights = floats(v[2], R, x);
+    float* loss = floats(v[4], 1, x);
+    const float* ref = floats(v[9], R, x);
+    float *sums = floats(v[13], S, x), *logp = floats(v[14], R, x);
+    want(loss != nullptr);
+    const at::Tensor* grad = nullptr;
+    if (v[11] == Py_True) {
+      grad = none(v[12]) ? &x : &tensor(v[12]);
+      want(on(*grad, x) && grad->scalar_type() == x.scalar_type() && grad->sizes() == x.sizes() && logits_rows(*grad) == f32);
+    } else {
+      want(none(v[12]));
+    }
+    const auto options = x.options().dtype(at::kFloat).requires_grad(false);
+    at::Tensor work = empty({6 * R + S + 1 + (logp == nullptr ? R : 0)}, options);
+    float* w = static_cast<float*>(work.data_ptr());
+    if (logp == nullptr) logp = w + 6 * R + S + 1;
+    launch(grad == nullptr ? PREFERENCE : PREFERENCE_GRAD, ss_preference, x.data_ptr(), f32, pitch(x),
+           static_cast<const long long*>(targets.data_ptr()), weights, static_cast<const int*>(cu.data_ptr()), R, V, S / 2, ref,
+           static_cast<float>(beta), kind, static_cast<float>(smoothing), v[8] == Py_True, static_cast<float>(number(v[10])), logp, sums,
+           loss, grad == nullptr ? nullptr : grad->data_ptr(), grad == nullptr ? 0 : pitch(*grad), w, stream);
+    Py_INCREF(v[4]);
+    return v[4];
+  });
+}
+
+// adamw8_many(list of (p, g, m, r, m_exp, r_exp, offset), (lr, beta1, beta2, eps, weight_decay, grad_scale), step, seed,
+//             stochastic_param, stochastic_state) -> None
+PyObject* adamw8_many(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 6, [&]() -> PyObject* {
+    want(PyList_CheckExact(v[0]) && PyTuple_CheckExact(v[1]) && PyTuple_GET_SIZE(v[1]) == 6 && PyList_GET_SIZE(v[0]) > 0);
+    const Py_ssize_t count = PyList_GET_SIZE(v[0]);
+    std::vector<long long> table;
+    std::vector<const void*> parameters;
+    table.reserve(8 * count);
+    void* stream = nullptr;
+    at::ScalarType types[2] = {at::kFloat, at::kFloat};
+    const at::Tensor* first = nullptr;
+    for (Py_ssize_t i = 0; i < count; ++i) {
+      PyObject* item = PyList_GET_ITEM(v[0], i);
+      want(PyTuple_CheckExact(item) && PyTuple_GET_SIZE(item) == 7);
+      const at::Tensor* t[6];
+      for (int j = 0; j < 6; ++j) t[j] = &tensor(PyTuple_GET_ITEM(item, j));
+      const long long offset = integer(PyTuple_GET_ITEM(item, 6));
+      if (first == nullptr) {
+        first = t[0];
+        stream = stream_of(*first);
+        for (int j = 0; j < 2; ++j) types[j] = t[j]->scalar_type();
+      }
+      const int64_t elements = t[0]->numel(), blocks = (elements + 255) / 256;
+      for (int j = 0; j < 6; ++j) {
+        const at::ScalarType type = j < 2 ? types[j] : j < 4 ? at::kFloat8_e4m3fn : at::kByte;
+        want(on(*t[j], *first) && t[j]->scalar_type() == type && t[j]->is_contiguous() && t[j]->numel() == (j < 4 ? elements : blocks));
+      }
+      want((types[0] == at::kFloat || types[0] == at::kBFloat16) && (types[1] == at::kFloat || types[1] == at::kBFloat16) &&
+           offset >= 0 && offset % 8 == 0);
+      for (int j = 0; j < 6; ++j) table.push_back(reinterpret_cast<long long>(t[j]->data_ptr()));
+      table.push_back(elements);
+      table.push_back(offset);
+      if (elements) parameters.push_back(t[0]->data_ptr());
+    }
+    std::sort(parameters.begin(), parameters.end());
+    want(std::adjacent_find(parameters.begin(), parameters.end()) == parameters.end());       // twice the same: in order, in Python
+    double hyper[6];
+    for (int j = 0; j < 6; ++j) hyper[j] = number(PyTuple_GET_ITEM(v[1], j));
+    const long long step = integer(v[2]);
+    want(step >= 1 && step <= INT_MAX);
+    launch(ADAMW8, ss_adamw8_many, table.data(), count, types[0] == at::kFloat, types[1] == at::kFloat, hyper, step, integer(v[3]),
+           v[4] == Py_True, v[5] == Py_True, stream);
+    Py_RETURN_NONE;
+  });
+}
+
 // set_status(device, address)
 PyObject* set_status(PyObject*, PyObject* const* v, Py_ssize_t n) {
   return guarded(n, 2, [&]() -> PyObject* {
@@ -352,7 +508,8 @@ PyObject* launched(PyObject*, PyObject* const*, Py_ssize_t n) {
 #define SS_CALL(name) {#name, reinterpret_cast<PyCFunction>(name), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {SS_CALL(gemm), SS_CALL(linear_residual), SS_CALL(swiglu_linear), SS_CALL(swiglu_linear_dgrad),
                          SS_CALL(rmsnorm_fwd), SS_CALL(rmsnorm_bwd), SS_CALL(rope), SS_CALL(attention_fwd),
-                         SS_CALL(attention_bwd), SS_CALL(set_status), SS_CALL(launched), {nullptr, nullptr, 0, nullptr}};
+                         SS_CALL(attention_bwd), SS_CALL(select_experts), SS_CALL(select_experts_bwd),
+                         SS_CALL(preference), SS_CALL(adamw8_many), SS_CALL(set_status), SS_CALL(launched), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_calls", nullptr, -1, methods};
 
 }  // namespace

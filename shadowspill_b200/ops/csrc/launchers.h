@@ -36,4 +36,18 @@ int ss_attn_bwd_g(const void* q, const void* k, const void* v, const void* out, 
                   void* dk, void* dv, const int* cu_seqlens, float* delta_scratch, int nseq, int T, int Hq, int Hkv, int dh,
                   long long ldq, long long ldk, long long ldv, long long ldo, long long lddq, long long lddk, long long lddv,
                   float scale, int* status, void* stream);
+// routing.cu
+int ss_select_experts(const void* logits, int bf16_logits, long long ld, const float* bias, int T, int E, int k, int groups,
+                      int keep_groups, int sigmoid, int renormalize, float scale, int* ids, float* weights, int* counts,
+                      void* stream);
+int ss_select_experts_bwd(const void* logits, int bf16_logits, long long ld, const int* ids, const float* dweights, int T, int E,
+                          int k, int sigmoid, int renormalize, float scale, void* dlogits, void* stream);
+// preference.cu
+int ss_preference(const void* logits, int fp32_logits, long long ld, const long long* targets, const float* weights,
+                  const int* cu_seqlens, int R, int V, int pairs, const float* ref_logp, float beta, int kind, float smoothing,
+                  int average, float grad_scale, float* logp, float* sums, float* loss_sum, void* grad, long long ldg, void* work,
+                  void* stream);
+// adamw8.cu
+int ss_adamw8_many(const long long* tensors, int count, int p_f32, int g_f32, const double* hyper, int step, long long seed,
+                   int sr_param, int sr_state, void* stream);
 }

@@ -16,6 +16,7 @@
 #include <type_traits>
 
 #include "chained_launch.cuh"
+#include "launchers.h"
 
 namespace ss {
 namespace {

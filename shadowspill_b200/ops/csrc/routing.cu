@@ -16,6 +16,8 @@
 
 #include <type_traits>
 
+#include "launchers.h"
+
 namespace ss {
 namespace {
 

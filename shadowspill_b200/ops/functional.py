@@ -493,6 +493,12 @@ def preference_(logits, targets, weights, cu_seqlens, loss_sum, *, beta=0.1, kin
     count for nothing and are not read; a pair with a side of only such rows has no loss. They, and rows of no sequence,
     get a gradient of zero. ``sums`` (fp32, one per sequence) receives the log ratios and ``logp`` (fp32[R]) the rows'
     log-probabilities, 0 where nothing is scored."""
+    host = _host(logits)
+    if host is not None and kind in reference.PREFERENCE_KINDS:
+        got = host.preference(logits, targets, weights, cu_seqlens, loss_sum, beta, reference.PREFERENCE_KINDS.index(kind),
+                              label_smoothing, bool(average), ref_logp, grad_scale, bool(write_grad), grad, sums, logp)
+        if got is not NotImplemented:
+            return got
     R, V = logits.shape
     if kind not in reference.PREFERENCE_KINDS:
         raise ValueError(f"unknown preference loss {kind!r}; known: {reference.PREFERENCE_KINDS}")
@@ -643,6 +649,13 @@ def adamw8_many_(tensors, *, lr, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0
     rounded stochastically, like bf16 parameters, by a counter RNG keyed on (seed, step, offset + element), or to nearest;
     moments rounded to nearest stop following a gradient whose size changes by less than a code's step. A tensor may be updated
     in parts that start on whole blocks, with the same bits. On the CPU all roundings are to nearest."""
+    tensors = list(tensors)
+    host = _host(tensors[0][0]) if tensors else None
+    if host is not None:
+        got = host.adamw8_many(tensors, (lr, beta1, beta2, eps, weight_decay, grad_scale), step, seed, bool(stochastic_param),
+                               bool(stochastic_state))
+        if got is not NotImplemented:
+            return
     if step < 1:
         raise ValueError("steps count from 1")
     hyper = dict(lr=lr, beta1=beta1, beta2=beta2, eps=eps, weight_decay=weight_decay, step=step, grad_scale=grad_scale)
@@ -654,8 +667,8 @@ def adamw8_many_(tensors, *, lr, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0
             with _device_of(where):
                 _lib.check(_lib.lib().ss_adamw8_many(
                     (ctypes.c_longlong * len(table))(*table), len(table) // 8, int(p_dtype == torch.float32),
-                    int(g_dtype == torch.float32), lr, beta1, beta2, eps, weight_decay, step, grad_scale, seed,
-                    int(stochastic_param), int(stochastic_state), _lib.stream_ptr()), "ss_adamw8_many")
+                    int(g_dtype == torch.float32), (ctypes.c_double * 6)(lr, beta1, beta2, eps, weight_decay, grad_scale), step,
+                    seed, int(stochastic_param), int(stochastic_state), _lib.stream_ptr()), "ss_adamw8_many")
         tables.clear()
         seen.clear()
 

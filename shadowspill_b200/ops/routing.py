@@ -42,6 +42,11 @@ def select_experts(logits: torch.Tensor, k: int, *, scoring: str = "softmax", bi
     -inf or NaN come last, so that the ids of a token are always ``k`` different experts. The weights are the picks' scores
     (without the bias), divided by their sum (+ 1e-20) if ``renormalize``, times ``scale``; a token whose logits are all -inf
     gets weights of zero under softmax, one with a NaN or +inf gets NaN."""
+    host = F._host(logits)
+    if host is not None:
+        got = host.select_experts(logits, k, _SIGMOID.get(scoring, -1), bias, groups, keep_groups, bool(renormalize), scale)
+        if got is not NotImplemented:
+            return got
     _check(logits, k, scoring, groups, keep_groups)
     T, E = logits.shape
     if bias is not None and (bias.shape != (E,) or bias.dtype != torch.float32 or bias.device != logits.device):
@@ -68,6 +73,11 @@ def select_experts_bwd(logits: torch.Tensor, ids: torch.Tensor, dweights: torch.
                        renormalize: bool = True, scale: float = 1.0) -> torch.Tensor:
     """Gradient of ``select_experts``'s weights (``dweights`` fp32 [T,k]) as a gradient of the logits, in their type; the
     picks and the bias are constants."""
+    host = F._host(logits)
+    if host is not None:
+        got = host.select_experts_bwd(logits, ids, dweights, _SIGMOID.get(scoring, -1), bool(renormalize), scale)
+        if got is not NotImplemented:
+            return got
     if ids.dim() != 2 or ids.dtype != torch.int32 or dweights.shape != ids.shape or ids.shape[0] != logits.shape[0]:
         raise ValueError("ids are int32 [T, k] and dweights has their shape")
     if ids.device != logits.device or dweights.device != logits.device:
