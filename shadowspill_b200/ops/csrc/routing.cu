@@ -5,8 +5,8 @@
 //   the best groups are the picks, ties to the lowest index; w_j = scale s_j / (sum_i s_i + 1e-20), or scale s_j.
 //
 // Which experts are picked is defined by keys in 64 bits. The kernel forms them in 32 and looks at the gaps between the picks,
-// to the best key left over, and between the groups kept and dropped: a token with a gap within the error of its keys is
-// done again in 64 bits. Where nothing is added to the scores and there are no groups the logits themselves are compared,
+// to the best key left over, and between the groups kept and dropped: where a gap is within the error of its keys, the groups or the
+// candidates are compared again in 64 bits. Where nothing is added to the scores and there are no groups the logits themselves are compared,
 // which needs neither.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -42,11 +42,13 @@ __device__ __forceinline__ float warp_max32(float v) {
 }
 
 // exp and 1 / (1 + exp(-x)) without the steps that keep denormal results.
-__device__ __forceinline__ float exp_of(float x) {
+constexpr float LOG2E = 1.44269504f;
+__device__ __forceinline__ float ex2(float x) {
   float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * 1.44269504f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
   return e;
 }
+__device__ __forceinline__ float exp_of(float x) { return ex2(x * LOG2E); }
 __device__ __forceinline__ float sigmoid_of(float x) {
   float s;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + exp_of(-x)));
@@ -106,45 +108,56 @@ __device__ unsigned kept_groups(const F* keys, const RouteArgs& a, int lane, F& 
   return bits;
 }
 
-// The picks with keys in 64 bits; lane j returns the j-th.
-template <int PER, class L>
-__device__ __noinline__ int picks_exact(const L* row, const RouteArgs& a, const unsigned char* group_of, double* keys, int lane) {
+// A row's largest logit and its softmax's sum in 64 bits, of the lanes' own values where LANES share a row.
+template <int LANES>
+__device__ __forceinline__ double sum64(float top, double part) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) part += __shfl_xor_sync(FULL, part, o);
+  return top > -INFINITY ? part : 1.0;
+}
+__device__ __forceinline__ double key64(float x, float top, double total, const float* bias, int e, bool sigmoid) {
+  double v = sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(x))) : x == -INFINITY ? 0.0 : exp(static_cast<double>(x) - top) / total;
+  if (bias != nullptr) v += bias[e];
+  return v == v ? v : -INFINITY;
+}
+
+// All keys of a row in 64 bits into shared memory, by a whole warp, and the groups that stay, as bits.
+template <class L>
+__device__ __noinline__ unsigned exact_keys(const L* row, const RouteArgs& a, double* keys, int lane) {
   float top = -INFINITY;
   for (int e = lane; e < a.E; e += 32) top = fmaxf(top, load_logit(row + e));
   top = warp_max32(top);
-  double total = 0.0;
-  if (!a.sigmoid) {
+  double part = 0.0;
+  if (!a.sigmoid)
     for (int e = lane; e < a.E; e += 32) {
       const float x = load_logit(row + e);
-      if (x > -INFINITY) total += exp(static_cast<double>(x) - top);
+      if (x > -INFINITY) part += exp(static_cast<double>(x) - top);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(FULL, total, o);
-  }
-  for (int e = lane; e < a.E; e += 32) {
-    const double x = load_logit(row + e);
-    double v = a.sigmoid ? 1.0 / (1.0 + exp(-x)) : (x > -INFINITY ? exp(x - top) / total : x * 0.0);
-    if (!a.sigmoid && x == -INFINITY) v = 0.0;
-    if (a.bias != nullptr) v += a.bias[e];
-    keys[e] = v == v ? v : -INFINITY;
-  }
+  const double total = sum64<32>(top, part);
+  for (int e = lane; e < a.E; e += 32) keys[e] = key64(load_logit(row + e), top, total, a.bias, e, a.sigmoid);
   __syncwarp();
+  unsigned bits = FULL;
   if (a.groups > 1) {
     double gap;
-    const unsigned bits = kept_groups(keys, a, lane, gap);
-    __syncwarp();
-    for (int e = lane; e < a.E; e += 32)
-      if (!((bits >> group_of[e]) & 1)) keys[e] = -INFINITY;
+    bits = kept_groups(keys, a, lane, gap);
     __syncwarp();
   }
+  return bits;
+}
+
+// The picks among those keys; lane j returns the j-th.
+__device__ __noinline__ int picks_exact(const RouteArgs& a, unsigned bits, const unsigned char* group_of, double* keys, int lane) {
+  for (int e = lane; e < a.E; e += 32)
+    if (!((bits >> group_of[e]) & 1)) keys[e] = -INFINITY;
+  __syncwarp();
   unsigned taken = 0;                            // this lane's experts that are picked, by place
   int mine = 0;
   for (int j = 0; j < a.k; ++j) {
     double best = -INFINITY;
     int at = INT_MAX;
-    for (int i = 0; i < PER; ++i) {
+    for (int i = 0; lane + 32 * i < a.E; ++i) {
       const int e = lane + 32 * i;
-      if (e < a.E && !((taken >> i) & 1) && (at == INT_MAX || keys[e] > best)) { best = keys[e]; at = e; }
+      if (!((taken >> i) & 1) && (at == INT_MAX || keys[e] > best)) { best = keys[e]; at = e; }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -157,6 +170,28 @@ __device__ __noinline__ int picks_exact(const L* row, const RouteArgs& a, const 
   }
   __syncwarp();
   return mine;
+}
+
+// Among the `n` candidates of a token, one to a lane (`id`, or -1), the number that come before this lane's by keys in 64 bits.
+// `top`: the row's largest logit; `most`: the largest n of the warp.
+template <int LANES, class L>
+__device__ __noinline__ int exact_places(const L* row, const RouteArgs& a, float top, int lane, int id, int n, int most) {
+  const int rank = lane % LANES, base = lane - rank;
+  double part = 0.0;
+  if (!a.sigmoid)
+    for (int e = rank; e < a.E; e += LANES) {
+      const float x = load_logit(row + e);
+      if (x > -INFINITY) part += exp(static_cast<double>(x) - top);
+    }
+  const double total = sum64<LANES>(top, part);
+  const double mine = id >= 0 ? key64(load_logit(row + id), top, total, a.bias, id, a.sigmoid) : -INFINITY;
+  int ahead = 0;
+  for (int c = 0; c < most; ++c) {
+    const double other = __shfl_sync(FULL, mine, base + min(c, LANES - 1));
+    const int whose = __shfl_sync(FULL, id, base + min(c, LANES - 1));
+    ahead += c < n && (other > mine || (other == mine && whose < id));
+  }
+  return ahead;
 }
 
 // PER consecutive values of a row from expert `first` on, -inf behind the last expert.
@@ -183,7 +218,8 @@ __device__ __forceinline__ void load_row(const L* row, int first, int E, bool ve
 //
 // The k-th largest of the lanes' own maxima bounds the k-th largest key from below: the keys from it on, a dozen where k
 // is 8, are gathered by one place to a lane and sorted. Where they are more than the lanes (one token in twenty for k = 8 of 16
-// lanes; many equal keys), or fewer than k can be compared, the picks are taken one by one instead.
+// lanes; many equal keys), or fewer than k can be compared, the picks are taken one by one instead. A doubt among those is settled
+// over the whole row, one among the gathered, which hold whatever may come before the k-th, between them.
 constexpr int rt_resident(int per) { return per == 16 ? 7 : 8; }     // blocks that an SM's registers hold
 template <int LANES, int PER, bool LOGITS, class L>
 __global__ void __launch_bounds__(RT_THREADS, rt_resident(PER))
@@ -204,6 +240,14 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, bool bias_vect
   }
   __syncthreads();
   double* const keys64 = warp_keys + warp * a.E;
+  unsigned ups = 0;                              // the sorting steps in which this lane keeps the larger of two
+  {
+    int step = 0;
+#pragma unroll
+    for (int n = 2; n <= LANES; n *= 2)
+#pragma unroll
+      for (int o = n / 2; o > 0; o >>= 1, ++step) ups |= static_cast<unsigned>(((rank & n) == 0) == ((rank & o) == 0)) << step;
+  }
   const int tokens = gridDim.x * RT_WARPS * TOKENS;
   for (int t0 = (blockIdx.x * RT_WARPS + warp) * TOKENS; t0 < a.T; t0 += tokens) {
     const int t = t0 + base / LANES;
@@ -214,12 +258,12 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, bool bias_vect
     load_row<PER>(row, first, a.E, vectors, v);
     float top = 0.f, total = 1.f;
     bool bad = false;                            // a softmax with a NaN or +inf in it
-    if (!a.sigmoid) {
+    const bool whole = !a.sigmoid && !(LOGITS && a.renormalize);         // the softmax's sum is needed
+    if (!a.sigmoid && !whole) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) bad = bad || !(v[i] < INFINITY);
       bad = (__ballot_sync(FULL, bad) & own) != 0;
     }
-    const bool whole = !a.sigmoid && !(LOGITS && a.renormalize);         // the softmax's sum is needed
     if (whole) {
       top = v[0];
 #pragma unroll
@@ -236,14 +280,16 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, bool bias_vect
       }
 #pragma unroll
       for (int o = LANES / 2; o > 0; o >>= 1) total += __shfl_xor_sync(FULL, total, o);
+      bad = !(total < INFINITY);                 // exponentials of NaN and of inf - inf
       total = fmaxf(total, 1.f);                 // the largest alone is 1
     }
     // v becomes the keys: -inf for what cannot be picked or compared
     float slack = 0.f;
     if (!LOGITS) {
-      // errors of a key: the score's (a relative 2^-21 of the largest: exp, its sum, the division) and the sum's rounding
+      // errors of a key before its sum is rounded. sigmoid: exp's |x| 6e-8 + 2.4e-7 times s (1 - s), the reciprocal's 6e-8 s and the
+      // sum 1 + exp's as much; softmax: exp's times exp(-|x|), its sum's and the reciprocal's, 4e-7 together, of the largest
       const float inv = __fdividef(1.f, total);
-      slack = a.sigmoid ? 1.5e-6f : 1.5e-6f * inv;
+      slack = a.sigmoid ? 3e-7f : 1e-6f * inv;
       float b[PER];
       if (a.bias != nullptr) load_row<PER>(a.bias, first, a.E, bias_vectors, b);
 #pragma unroll
@@ -255,8 +301,8 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, bool bias_vect
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i) v[i] = fmaxf(v[i], -INFINITY);         // NaN
-    bool again = false;
     if (!LOGITS && a.groups > 1) {
+      unsigned stay = 0;
       float gap, big;                            // big: the largest of the keys that group scores are sums of
       if (lane_groups) {
         float best = -INFINITY, second = -INFINITY;
@@ -287,13 +333,9 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, bool bias_vect
           big = fmaxf(big, __shfl_xor_sync(FULL, big, o));
         }
         gap = worst - left;
-        if (!kept) {
-#pragma unroll
-          for (int i = 0; i < PER; ++i) v[i] = -INFINITY;
-        }
+        stay = kept ? 1u << group : 0u;          // this lane's own group
       } else {
         float* keys = reinterpret_cast<float*>(keys64);
-        unsigned bits = 0;
         gap = big = 0.f;
 #pragma unroll
         for (int i = 0; i < PER; ++i) big = fmaxf(big, v[i] > -INFINITY ? fabsf(v[i]) : 0.f);
@@ -308,26 +350,41 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, bool bias_vect
           __syncwarp();
           float g;
           const unsigned b = kept_groups(keys, a, lane, g);
-          if (base == part * LANES) { bits = b; gap = g; }
+          if (base == part * LANES) { stay = b; gap = g; }
           __syncwarp();
         }
+      }
+      const bool doubtful = a.keep < a.groups && !(gap > 4.f * slack + 5e-7f * big);
+      unsigned redo = __ballot_sync(FULL, doubtful && rank == 0 && real);
+      while (redo) {                             // the whole warp, token by token: the groups by keys in 64 bits
+        const int at = __ffs(redo) - 1;
+        redo &= redo - 1;
+        const unsigned bits = exact_keys(logits + static_cast<long long>(t0 + at / LANES) * a.ld, a, keys64, lane);
+        if (base == at) stay = bits;
+        __syncwarp();
+      }
+      if (lane_groups) {
+        if (!((stay >> (rank / group_lanes)) & 1)) {
+#pragma unroll
+          for (int i = 0; i < PER; ++i) v[i] = -INFINITY;
+        }
+      } else {
 #pragma unroll
         for (int i = 0; i < PER; ++i)
-          if (first + i < a.E && !((bits >> group_of[first + i]) & 1)) v[i] = -INFINITY;
+          if (first + i < a.E && !((stay >> group_of[first + i]) & 1)) v[i] = -INFINITY;
       }
-      again = a.keep < a.groups && !(gap > 4.f * slack + 5e-7f * big);
     }
     // the k-th largest of the lanes' maxima
     float most = v[0];
 #pragma unroll
     for (int i = 1; i < PER; ++i) most = fmaxf(most, v[i]);
+    int step = 0;
 #pragma unroll
     for (int n = 2; n <= LANES; n *= 2)
 #pragma unroll
-      for (int o = n / 2; o > 0; o >>= 1) {
+      for (int o = n / 2; o > 0; o >>= 1, ++step) {
         const float other = __shfl_xor_sync(FULL, most, o);
-        const bool up = (((rank & n) == 0) == ((rank & o) == 0));          // this lane keeps the larger
-        most = up ? fmaxf(most, other) : fminf(most, other);
+        most = (ups >> step) & 1 ? fmaxf(most, other) : fminf(most, other);
       }
     const float least = __shfl_sync(FULL, most, base + min(a.k, LANES) - 1);
     const float from = LOGITS ? least : least - (2.f * slack + 2.5e-7f * fabsf(least));      // and what an error may put before it
@@ -345,7 +402,7 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, bool bias_vect
       all = __shfl_sync(FULL, place, base + LANES - 1);
       place -= n;
     }
-    const bool sorted = least > -INFINITY && all <= LANES && a.k <= LANES;
+    const bool sorted = least > -INFINITY && all >= a.k && all <= LANES;     // a key of inf leaves nothing to choose by
     int mine = 0;
     if (__any_sync(FULL, sorted)) {
       if (sorted) {
@@ -356,36 +413,44 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, bool bias_vect
       __syncwarp();
       float key = -INFINITY;
       int id = INT_MAX;
-      if (sorted && rank < all) {
+      const bool holds = sorted && rank < all;
+      if (holds) {
         const float2 c = gathered[warp][lane];
         key = c.x;
         id = __float_as_int(c.y);
       }
       __syncwarp();
+      step = 0;
 #pragma unroll
       for (int n = 2; n <= LANES; n *= 2)
 #pragma unroll
-        for (int o = n / 2; o > 0; o >>= 1) {
+        for (int o = n / 2; o > 0; o >>= 1, ++step) {
           const float other = __shfl_xor_sync(FULL, key, o);
           const int whose = __shfl_xor_sync(FULL, id, o);
-          const bool up = (((rank & n) == 0) == ((rank & o) == 0));
           const bool ahead = other > key || (other == key && whose < id);
-          if (ahead == up) { key = other; id = whose; }
+          if (ahead == static_cast<bool>((ups >> step) & 1)) { key = other; id = whose; }
         }
-      mine = id;
       if (!LOGITS) {
         const float next = __shfl_down_sync(FULL, key, 1, LANES);
-        const bool close = rank < a.k && rank + 1 < all && key - next <= 2.f * slack + 2.5e-7f * fabsf(key);
-        const unsigned near = __ballot_sync(FULL, close && sorted);        // all lanes of the warp take part, whatever `again` is
-        again = again || (near & own) != 0;
+        const bool close = holds && rank < a.k && rank + 1 < all && key - next <= 2.f * slack + 2.5e-7f * fabsf(key);
+        const unsigned near = __ballot_sync(FULL, close);
+        if (near != 0) {                         // some pick of the warp's is in doubt: the candidates again, by their keys in 64 bits
+          const int n = sorted ? all : 0, most_of = LANES == 32 ? n : max(n, __shfl_xor_sync(FULL, n, 16));
+          const int ahead = exact_places<LANES>(row, a, top, lane, holds ? id : -1, n, most_of);
+          if (holds) gathered[warp][base + ahead].y = __int_as_float(id);
+          __syncwarp();
+          if (holds) id = __float_as_int(gathered[warp][lane].y);
+        }
       }
+      __syncwarp();                              // the next token's candidates come into the same place
+      mine = id;
     }
-    const bool one_by_one = LOGITS && !sorted;
-    if (!LOGITS) again = again || !sorted;
-    if (LOGITS && __any_sync(FULL, one_by_one)) {
+    const bool one_by_one = !sorted;
+    bool doubt = false;
+    if (__any_sync(FULL, one_by_one)) {
       float last_key = INFINITY;                 // the pick before, of those that compare, then of the rest
       int last_id = -1, left = -1, found = -1;
-      for (int j = 0; j < a.k; ++j) {
+      for (int j = 0; j < a.k + !LOGITS; ++j) {  // one more where the last pick's lead counts
         float best = -INFINITY;                  // the largest behind the last pick
         int at = INT_MAX;
 #pragma unroll
@@ -399,14 +464,17 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, bool bias_vect
           const int w = __shfl_xor_sync(FULL, at, o);
           if (b > best || (b == best && w < at)) { best = b; at = w; }
         }
+        if (!LOGITS) doubt = doubt || (best == -INFINITY ? j < a.k : last_key - best <= 2.f * slack + 2.5e-7f * fabsf(best));
         // nothing left that compares: the first experts that do not, in their order (looked for by all lanes: the warp's tokens
         // differ in this)
         int rest = INT_MAX;
+        if (LOGITS) {
 #pragma unroll
-        for (int i = PER - 1; i >= 0; --i)
-          if (first + i < a.E && v[i] == -INFINITY && first + i > left) rest = first + i;
+          for (int i = PER - 1; i >= 0; --i)
+            if (first + i < a.E && v[i] == -INFINITY && first + i > left) rest = first + i;
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) rest = min(rest, __shfl_xor_sync(FULL, rest, o));
+          for (int o = LANES / 2; o > 0; o >>= 1) rest = min(rest, __shfl_xor_sync(FULL, rest, o));
+        }
         if (best == -INFINITY) {
           at = left = rest;
         } else {
@@ -418,11 +486,12 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, bool bias_vect
       if (one_by_one) mine = found;
     }
     if (!LOGITS) {
-      unsigned redo = __ballot_sync(FULL, again && rank == 0 && real);
+      unsigned redo = __ballot_sync(FULL, one_by_one && doubt && rank == 0 && real);
       while (redo) {                             // the whole warp, token by token
         const int at = __ffs(redo) - 1;
         redo &= redo - 1;
-        const int pick = picks_exact<RT_MAX_E / 32>(logits + static_cast<long long>(t0 + at / LANES) * a.ld, a, group_of, keys64, lane);
+        const unsigned bits = exact_keys(logits + static_cast<long long>(t0 + at / LANES) * a.ld, a, keys64, lane);
+        const int pick = picks_exact(a, bits, group_of, keys64, lane);
         const int moved = __shfl_sync(FULL, pick, rank);
         if (base == at) mine = moved;
       }
@@ -528,8 +597,11 @@ int ss_select_experts(const void* logits, int bf16_logits, long long ld, const f
   const RouteArgs a{T, E, k, groups, keep_groups, sigmoid, renormalize, ld, scale, bias};
   if (!fits(a)) return -2;
   cudaStream_t s = (cudaStream_t)stream;
-  // Half a warp to a token where it has twice as many lanes as picks, with up to 16 experts to a lane.
-  const bool halves = 2 * k <= 16 && E <= 256;
+  const bool plain = bias == nullptr && groups == 1;
+  // Half a warp to a token where the candidates are hardly ever more than its lanes: a token too many in twenty at k = 8 of 16
+  // costs little where logits are compared, but what is doubtful of it is settled over a whole row, which the launch waits for (8,192
+  // tokens, k = 8: 64 experts by logits 10.1 us, with whole warps 12.6; 256 with a bias 24.5, with whole warps 19.9).
+  const bool halves = (plain ? 2 : 3) * k * groups <= 16 * keep_groups && E <= 256;
   const int lanes = halves ? 16 : 32, per_block = RT_WARPS * (halves ? 2 : 1);
   const int per = (E + lanes - 1) / lanes, most = 148 * rt_resident(per <= 8 ? 8 : 16);
   const int blocks = (T + per_block - 1) / per_block, grid = blocks < 1 ? 1 : blocks < most ? blocks : most;
@@ -537,7 +609,6 @@ int ss_select_experts(const void* logits, int bf16_logits, long long ld, const f
     const cudaError_t e = cudaMemsetAsync(counts, 0, sizeof(int) * E, s);
     if (e != cudaSuccess) return (int)e;
   }
-  const bool plain = bias == nullptr && groups == 1;
   auto go = [&](auto kern, auto* x) {
     const bool vectors = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld * sizeof(*x) % 16 == 0;
     kern<<<grid, RT_THREADS, plain ? 0 : sizeof(double) * E * RT_WARPS, s>>>(x, vectors, reinterpret_cast<uintptr_t>(bias) % 16 == 0, a, ids, weights, counts);
