@@ -87,15 +87,12 @@ class _Norms:
         if c.router_scoring == "sigmoid":
             # scores in (0, 1); a frozen per-expert bias takes part in the selection only; the picked
             # scores are renormalised and scaled (GLM / DeepSeek-style routing without an auxiliary loss)
-            scores = torch.sigmoid(logits)
-            ids = torch.topk(scores + self.router_bias.float(), c.top_k, dim=-1).indices
-            picked = torch.gather(scores, 1, ids)
-            wts = picked / (picked.sum(-1, keepdim=True) + 1e-20) * c.routed_scaling_factor
+            ids, wts = S.select_experts(logits, self.router_bias.float(), c.top_k, True, 1, 1, True, float(c.routed_scaling_factor))
             if "w13" in self.adapted:
-                out = S.moe_experts_routed_lora(h, ids.to(torch.int32), wts, self.w13, self.w2, self.w13_lora_a,
+                out = S.moe_experts_routed_lora(h, ids, wts, self.w13, self.w2, self.w13_lora_a,
                                                 self.w13_lora_b, self.w2_lora_a, self.w2_lora_b, float(self.lora.scale))
             else:
-                out = S.moe_experts_routed(h, ids.to(torch.int32), wts, self.w13, self.w2)
+                out = S.moe_experts_routed(h, ids, wts, self.w13, self.w2)
         elif "w13" in self.adapted:     # both banks carry per-expert factors (see graph_stage.supports)
             out = S.moe_experts_lora(h, logits, self.w13, self.w2, self.w13_lora_a, self.w13_lora_b,
                                      self.w2_lora_a, self.w2_lora_b, c.top_k, c.router_renormalize,

@@ -81,6 +81,8 @@ for _r in (
     OperatorRule("ss.moe_experts_routed_lora", "compute", None),
     OperatorRule("ss.sparse_latent_attention", "compute", None),
     OperatorRule("ss.index_topk", "compute", None),
+    OperatorRule("ss.select_experts", "memory", (0,)),
+    OperatorRule("ss.select_experts_bwd", "memory", (0, 1, 2)),
     OperatorRule("ss.rmsnorm", "memory", (0,)),
     OperatorRule("ss.rope", "memory", (0, 1)),
     OperatorRule("ss.swiglu", "memory", (0,)),

@@ -811,7 +811,54 @@ def _sla_bwd(ctx, gy):
 sparse_latent_attention.register_autograd(_sla_bwd, setup_context=_sla_setup)
 
 
+# ------------------------------------------------------------------------ selection of experts
+@custom_op("ss::select_experts", mutates_args=())
+def select_experts(logits: Tensor, bias: Tensor, k: int, sigmoid: bool, groups: int, keep_groups: int, renorm: bool,
+                   scale: float) -> tuple[Tensor, Tensor]:
+    """``routing.select_experts`` by rows: the picks and their weights (``bias`` only selects and is never trained)."""
+    from ..ops import routing
+    ids, wts, _ = routing.select_experts(logits, k, scoring="sigmoid" if sigmoid else "softmax", bias=bias, groups=groups,
+                                         keep_groups=keep_groups, renormalize=renorm, scale=scale)
+    return ids, wts
+
+
+@select_experts.register_fake
+def _(logits, bias, k, sigmoid, groups, keep_groups, renorm, scale):
+    return (logits.new_empty((logits.shape[0], k), dtype=torch.int32), logits.new_empty((logits.shape[0], k), dtype=torch.float32))
+
+
+@custom_op("ss::select_experts_bwd", mutates_args=())
+def select_experts_bwd(logits: Tensor, ids: Tensor, dwts: Tensor, sigmoid: bool, renorm: bool, scale: float) -> Tensor:
+    from ..ops import routing
+    return routing.select_experts_bwd(logits, ids, _c(dwts), scoring="sigmoid" if sigmoid else "softmax", renormalize=renorm, scale=scale)
+
+
+@select_experts_bwd.register_fake
+def _(logits, ids, dwts, sigmoid, renorm, scale):
+    return torch.empty_like(logits, memory_format=torch.contiguous_format)
+
+
+def _select_setup(ctx, inputs, output):
+    ctx.save_for_backward(inputs[0], output[0])
+    ctx.args = (inputs[3], inputs[6], inputs[7])
+
+
+def _select_bwd(ctx, _gids, gwts):
+    logits, ids = ctx.saved_tensors
+    return (torch.ops.ss.select_experts_bwd(logits, ids, gwts, *ctx.args), *(None,) * 7)
+
+
+select_experts.register_autograd(_select_bwd, setup_context=_select_setup)
+
+
 # ------------------------------------------------------------------------ routed experts, routing given
+def _counts(ids: Tensor, E: int) -> Tensor:
+    """How often each expert was picked, without a word to the host (``bincount`` waits for the largest pick)."""
+    flat = ids.reshape(-1).long()
+    return torch.zeros(E, dtype=torch.int32, device=ids.device).index_add_(
+        0, flat, torch.ones(1, dtype=torch.int32, device=ids.device).expand(flat.numel()))
+
+
 def _moe_routed_torch(h: Tensor, ids: Tensor, wts: Tensor, w13: Tensor, w2: Tensor) -> Tensor:
     """Top-k SwiGLU experts with the routing decided outside (``ids`` [T, k], ``wts`` [T, k]): the
     form for routers that are not a softmax (sigmoid scores with a selection-only bias)."""
@@ -839,7 +886,7 @@ def _moe_routed_torch(h: Tensor, ids: Tensor, wts: Tensor, w13: Tensor, w2: Tens
 def _moe_routed_cuda(h, ids, wts, w13, w2, sink):
     from ..models import autograd_ops as A
     from ..ops import moe as moe_ops
-    counts = torch.bincount(ids.reshape(-1).long(), minlength=w13.shape[0]).to(torch.int32)
+    counts = _counts(ids, w13.shape[0])
     lay = moe_ops.Layout(ids.to(torch.int32).contiguous(), counts)
     xs = A.expert_gather(h, lay)
     ys = A.grouped_linear(A.swiglu(A.grouped_linear(xs, w13, lay, sink, "w13")), w2, lay, sink, "w2")
@@ -925,7 +972,7 @@ def _moe_routed_lora_torch(h, ids, wts, w13, w2, a13, b13, a2, b2, scale: float)
 def _moe_routed_lora_cuda(h, ids, wts, w13, w2, a13, b13, a2, b2, scale: float, sink):
     from ..models import autograd_ops as A
     from ..ops import moe as moe_ops
-    counts = torch.bincount(ids.reshape(-1).long(), minlength=w13.shape[0]).to(torch.int32)
+    counts = _counts(ids, w13.shape[0])
     lay = moe_ops.Layout(ids.to(torch.int32).contiguous(), counts)
     xs = A.expert_gather(h, lay)
 

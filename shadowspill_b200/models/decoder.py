@@ -468,7 +468,11 @@ class HeadLossStage(Stage):
 
     def workspace_bytes(self, T, itemsize=2):
         c = self.cfg
-        return (min(T, self.block_rows) * c.vocab_size + 2 * T * c.d_model) * itemsize
+        return (min(T, self._block(T)) * c.vocab_size + 2 * T * c.d_model) * itemsize
+
+    def _block(self, T):
+        """Rows of logits formed at once: all of them for pairs, whose gradients wait for both of their sequences."""
+        return max(T, 1) if self.objective.kind == "preference" else self.block_rows
 
     def flops(self, T, mean_seqlen):
         return 2.0 * T * self.cfg.d_model * self.cfg.vocab_size
@@ -494,13 +498,13 @@ class HeadLossStage(Stage):
             w_first = first
         h, rstd = F.rmsnorm_fwd(x, P["final_norm"], c.norm_epsilon, c.zero_centered_norm)
         ob, X = self.objective, meta.extras
-        rows = token_head.scored(h, W, meta.targets, meta.weights, Gw)
+        rows = token_head.AllRows() if ob.kind == "preference" else token_head.scored(h, W, meta.targets, meta.weights, Gw)
         h = rows.take(h)
         dh = torch.empty_like(h) if train else None
         frozen = not G or "final_norm" not in G
         if train and first and not frozen:
             G["final_norm"].zero_()
-        B = self.block_rows
+        B = self._block(T)
         acc = not w_first
         for r0 in range(0, T, B):
             r1 = min(T, r0 + B)
@@ -510,6 +514,12 @@ class HeadLossStage(Stage):
                 rows.clipped_policy_(logits, meta.targets, meta.weights, X["old_logprobs"], X["advantages"], loss_sum,
                                      r0, r1, clip=ob.clip_ratio, ref_logp=ref, ref_beta=ob.reference_beta,
                                      grad_scale=grad_scale, write_grad=train)
+            elif ob.kind == "preference":
+                pairs = (meta.cu_seqlens.numel() - 1) // 2        # slots are an odd number in some geometries
+                F.preference_(logits, meta.targets, meta.weights, meta.cu_seqlens[:2 * pairs + 1], loss_sum,
+                              beta=ob.preference_beta, kind=ob.preference_loss, label_smoothing=ob.label_smoothing,
+                              average=ob.average_logprobs, grad_scale=grad_scale, write_grad=train,
+                              ref_logp=None if ob.reference_free else X["reference_logprobs"])
             else:
                 rows.cross_entropy_(logits, meta.targets, meta.weights, loss_sum, r0, r1, grad_scale=grad_scale,
                                     write_grad=train)

@@ -146,7 +146,10 @@ def _objective_record(rec: dict | None) -> dict | None:
     """Client ``Objective`` record (component id, config, summed terms) -> ``Objective`` JSON."""
     if not rec or rec.get("id", "shadowspill/cross_entropy@1") == "shadowspill/cross_entropy@1":
         return None
-    from ..models.objectives import Objective
+    from ..models.objectives import COMPONENT_IDS, Objective
+    if COMPONENT_IDS["preference"] in (rec["id"], *(t.get("id") for t in rec.get("terms", ()))):
+        # clients' datums are packed in an order of their own, which does not keep pairs side by side
+        raise ValueError("the preference objective is for in-process sessions, whose batches keep pairs adjacent")
     if rec["id"] == "shadowspill/sum@1":
         head, head_cfg, balance = "shadowspill/cross_entropy@1", {}, 0.0
         for term in rec.get("terms", ()):
