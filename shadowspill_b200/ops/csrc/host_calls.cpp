@@ -475,7 +475,7 @@ PyObject* adamw8_many(PyObject*, PyObject* const* v, Py_ssize_t n) {
     double hyper[6];
     for (int j = 0; j < 6; ++j) hyper[j] = number(PyTuple_GET_ITEM(v[1], j));
     const long long step = integer(v[2]);
-    want(step >= 1 && step <= INT_MAX);
+    want(step >= 1 && step <= INT_MAX && hyper[3] >= 1e-16);
     launch(ADAMW8, ss_adamw8_many, table.data(), count, types[0] == at::kFloat, types[1] == at::kFloat, hyper, step, integer(v[3]),
            v[4] == Py_True, v[5] == Py_True, stream);
     Py_RETURN_NONE;

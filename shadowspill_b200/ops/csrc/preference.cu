@@ -88,6 +88,17 @@ struct Rows {
     return t >= 0 && t < V && w != 0.f;
   }
   __device__ int bound(int i) const { return min(max(cu_seqlens[i], 0), R); }
+  // How many bounds are no larger than row r: by a warp, a 32nd of what is left at each step. In [0, 2 pairs + 1] whatever they hold.
+  __device__ int bounds_up_to(int r) const {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = 2 * pairs + 1;
+    while (lo < hi) {
+      const int step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step - 1;
+      lo += step * __popc(__ballot_sync(0xffffffffu, at < hi && bound(at) <= r));
+      hi = min(hi, lo + step - 1);
+    }
+    return lo;
+  }
 };
 struct PairArgs {
   float beta, smoothing, grad_scale;
@@ -179,6 +190,16 @@ __device__ __forceinline__ double team_sum64(double v, double* red) {
   return v;
 }
 
+// The pairs' losses in their order into the sum: by the team that has finished the last of them.
+template <int TEAM>
+__device__ void add_losses(const Rows& rows, const Work& work, float* loss_sum, double* red) {
+  __threadfence();
+  double total = 0.0;
+  for (int i = Team<TEAM>::rank(); i < rows.pairs; i += TEAM) total += __ldcg(work.pair_loss + i);
+  total = team_sum64<TEAM>(total, red);
+  if (Team<TEAM>::rank() == 0) *loss_sum += static_cast<float>(total);
+}
+
 // The loss of pair p from its rows' log ratios, and its rows' coefficients. By one team, when all rows are done. Sums are held
 // in 64 bits: they cancel between the two sides.
 template <int TEAM>
@@ -249,19 +270,32 @@ __device__ void finish_pair(int p, const Rows& rows, const PairArgs& a, const Wo
     if (rank == 0) *loss_sum += static_cast<float>(loss);
     return;
   }
-  // the block that finishes the last pair adds the pairs' losses, in their order
   bool last = false;
   if (rank == 0) {
     work.pair_loss[p] = static_cast<float>(loss);
     __threadfence();
     last = atomicAdd(work.pairs_done, 1) == rows.pairs - 1;
   }
-  if (!Team<TEAM>::any(last)) return;
+  if (Team<TEAM>::any(last)) add_losses<TEAM>(rows, work, loss_sum, red[0]);
+}
+
+// The pairs without rows, by one team.
+template <int TEAM>
+__device__ void finish_empty(const Rows& rows, const Work& work, float* sums, float* loss_sum, double* red) {
+  const int rank = Team<TEAM>::rank();
+  int empty = 0;
+  for (int p = rank; p < rows.pairs; p += TEAM) {
+    if (rows.bound(2 * p) < rows.bound(2 * p + 2)) continue;
+    if (sums != nullptr) sums[2 * p] = sums[2 * p + 1] = 0.f;
+    work.pair_loss[p] = 0.f;
+    ++empty;
+  }
   __threadfence();
-  double total = 0.0;
-  for (int i = rank; i < rows.pairs; i += TEAM) total += __ldcg(work.pair_loss + i);
-  total = team_sum64<TEAM>(total, red[0]);
-  if (rank == 0) *loss_sum += static_cast<float>(total);
+  Team<TEAM>::sync();
+  const int all = static_cast<int>(team_sum64<TEAM>(empty, red));
+  bool last = false;
+  if (rank == 0 && all > 0) last = atomicAdd(work.pairs_done, all) == rows.pairs - all;
+  if (Team<TEAM>::any(last)) add_losses<TEAM>(rows, work, loss_sum, red);
 }
 
 // A team per row, and one more for the pairs without rows.
@@ -273,16 +307,11 @@ preference_rows_kernel(const L* __restrict__ logits, long long ld, bool aligned,
   __shared__ double red_of[Team<TEAM>::ROWS][4][WARPS];
   __shared__ double parts[WARPS];                // of teams of several warps
   __shared__ float refs[WARPS], tops[WARPS];
-  __shared__ int counts[WARPS];
   const int rank = Team<TEAM>::rank(), row = Team<TEAM>::row();
   double (*red)[WARPS] = red_of[threadIdx.x / TEAM];
   if (row > rows.R) return;
   if (row == rows.R) {
-    for (int p = 0; p < rows.pairs; ++p)
-      if (rows.bound(2 * p) >= rows.bound(2 * p + 2)) {
-        finish_pair<TEAM>(p, rows, a, work, sums, loss_sum, red);
-        Team<TEAM>::sync();
-      }
+    finish_empty<TEAM>(rows, work, sums, loss_sum, red[0]);
     return;
   }
   long long target;
@@ -363,18 +392,7 @@ preference_rows_kernel(const L* __restrict__ logits, long long ld, bool aligned,
     logp[row] = 0.f;
     work.ratio[row] = 0.0;
   }
-  // the row's pair, by the number of bounds at or before it
-  int before = 0;
-  for (int i = rank; i < 2 * rows.pairs + 1; i += TEAM) before += rows.bound(i) <= row;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-  if (WARPS > 1) {
-    if ((rank & 31) == 0) counts[rank >> 5] = before;
-    __syncthreads();
-    before = 0;
-#pragma unroll
-    for (int i = 0; i < WARPS; ++i) before += counts[i];
-  }
+  const int before = rows.bounds_up_to(row);
   const int pair = before > 0 && before <= 2 * rows.pairs ? (before - 1) >> 1 : -1;
   bool last = false;
   if (rank == 0) {
@@ -510,7 +528,7 @@ int ss_preference(const void* logits, int fp32_logits, long long ld, const long 
                   const int* cu_seqlens, int R, int V, int pairs, const float* ref_logp, float beta, int kind, float smoothing,
                   int average, float grad_scale, float* logp, float* sums, float* loss_sum, void* grad, long long ldg, void* work,
                   void* stream) {
-  if (R < 0 || V < 1 || pairs < 0 || kind < 0 || kind > 2 || ld < V || (grad != nullptr && ldg < V)) return -2;
+  if (R < 0 || R > 0x7fff0000 || V < 1 || pairs < 0 || pairs > 0x3fffffff || kind < 0 || kind > 2 || ld < V || (grad != nullptr && ldg < V)) return -2;
   const Rows rows{targets, weights, ref_logp, cu_seqlens, R, V, pairs};
   const PairArgs a{beta, smoothing, grad_scale, kind, average};
   const long long n = R;

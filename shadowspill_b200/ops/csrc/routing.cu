@@ -102,7 +102,7 @@ __device__ unsigned kept_groups(const F* keys, const RouteArgs& a, int lane, F& 
     worst = w < worst ? w : worst;
     left = l > left ? l : left;
   }
-  gap = worst - left;                            // NaN where both are -inf: no gap
+  gap = worst < F(INFINITY) ? worst - left : F(NAN);         // NaN too where both are -inf: no gap
   unsigned bits = 0;
   for (int g = 0; g < a.groups; ++g) bits |= __shfl_sync(FULL, static_cast<unsigned>(kept), g * per) << g;
   return bits;
@@ -332,7 +332,7 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, bool bias_vect
           left = fmaxf(left, __shfl_xor_sync(FULL, left, o));
           big = fmaxf(big, __shfl_xor_sync(FULL, big, o));
         }
-        gap = worst - left;
+        gap = worst < INFINITY ? worst - left : NAN;         // a sum past the type's range says nothing
         stay = kept ? 1u << group : 0u;          // this lane's own group
       } else {
         float* keys = reinterpret_cast<float*>(keys64);
@@ -580,7 +580,7 @@ select_experts_bwd_kernel(const L* __restrict__ logits, RouteArgs a, const int* 
 }
 
 bool fits(const RouteArgs& a) {
-  return a.T >= 0 && a.E >= 1 && a.E <= RT_MAX_E && a.k >= 1 && a.k <= RT_MAX_K && a.k <= a.E && a.groups >= 1 &&
+  return a.T >= 0 && a.T <= 0x7fff0000 && a.E >= 1 && a.E <= RT_MAX_E && a.k >= 1 && a.k <= RT_MAX_K && a.k <= a.E && a.groups >= 1 &&
          a.groups <= RT_MAX_GROUPS && a.E % a.groups == 0 && a.keep >= 1 && a.keep <= a.groups &&
          a.k <= a.keep * (a.E / a.groups) && a.ld >= a.E;
 }

@@ -532,6 +532,8 @@ def preference_(logits, targets, weights, cu_seqlens, loss_sum, *, beta=0.1, kin
         raise TypeError("preference logits are bf16 or fp32 on CUDA")
     if logits.stride(1) != 1 or (out is not None and out.stride(1) != 1) or not (targets.is_contiguous() and cu_seqlens.is_contiguous()):
         raise ValueError("logits and their gradient have unit inner stride, targets and cu_seqlens are contiguous")
+    if R > 1 and (logits.stride(0) < V or (out is not None and out.stride(0) < V)):
+        raise ValueError("rows of logits and of their gradient do not overlap")
     with _device_of(logits):
         work = torch.empty(6 * R + S + 1, dtype=torch.float32, device=logits.device)
         lp = torch.empty(R, dtype=torch.float32, device=logits.device) if logp is None else logp
@@ -658,6 +660,8 @@ def adamw8_many_(tensors, *, lr, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0
             return
     if step < 1:
         raise ValueError("steps count from 1")
+    if not eps >= 1e-16:                    # roots under 1e-19 are flushed to zero
+        raise ValueError("eps is at least 1e-16 with 8-bit moments")
     hyper = dict(lr=lr, beta1=beta1, beta2=beta2, eps=eps, weight_decay=weight_decay, step=step, grad_scale=grad_scale)
     tables: dict = {}                       # (device, types) -> (a tensor there, eight numbers a tensor); insertion-ordered
     seen = set()

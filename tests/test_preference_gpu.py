@@ -194,6 +194,43 @@ def test_many_pairs_one_long_sequence_and_repeatable_bits():
     _compare(x, t, w, cu, ref_logp=ref, average=True)
 
 
+@pytest.mark.parametrize("V", [40, 3000])
+@pytest.mark.parametrize("pairs,most", [(16, 3), (513, 4), (5000, 2), (1, 40)])
+def test_pairs_by_the_hundred_with_empty_sides(pairs, most, V):
+    g = torch.Generator().manual_seed(pairs)
+    lengths = torch.randint(0, most + 1, (2 * pairs,), generator=g)
+    lengths[2:4] = 0                                              # a pair without rows
+    bounds = [0, *lengths.cumsum(0).tolist()]
+    x, t, w, cu, ref = _case(V, bounds, bounds[-1] + 3, seed=14, masked=0.1)
+    _compare(x, t, w, cu, ref_logp=ref, average=True)
+
+
+def test_rows_that_overlap_are_refused():
+    x, t, w, cu, ref = _case(64, [0, 4, 8], 8, seed=15)
+    loss = torch.zeros(1, device=DEV)
+    for bad in (dict(logits=x[:1].expand(8, 64)), dict(grad=x[:1].expand(8, 64)), dict(logits=x.t().contiguous().t())):
+        with pytest.raises(ValueError):
+            F.preference_(**{**dict(logits=x, targets=t, weights=w, cu_seqlens=cu, loss_sum=loss), **bad})
+    assert float(loss) == 0.0
+
+
+def test_two_streams_at_once():
+    cases = [_case(2000, [0, 300, 640], 640, seed=s) for s in (16, 17)]
+    want = [_compare(x, t, w, cu, ref_logp=ref) for x, t, w, cu, ref in cases]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[] for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, (x, t, w, cu, ref) in enumerate(cases):
+            with torch.cuda.stream(streams[i]):
+                loss, grad = torch.full((1,), 0.25, device=DEV), torch.empty_like(x)
+                F.preference_(x, t, w, cu, loss, grad=grad, ref_logp=ref)
+                got[i].append((loss, grad))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(loss, want[i][0]) and torch.equal(grad, want[i][2]) for loss, grad in got[i])
+
+
 def test_gradient_against_differences():
     x, t, w, cu, ref = _case(40, [0, 5, 9, 12, 20], 20, torch.float32, seed=9)
     grad = torch.empty_like(x)

@@ -111,6 +111,29 @@ def test_bad_logits_leave_different_experts_in_range(value, scoring, bias):
             assert bool(torch.isnan(w[bad]).all())
 
 
+@pytest.mark.parametrize("E,k", [(16, 4), (64, 8), (512, 10)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_biases_of_any_value(E, k, scoring):
+    """Experts forced in or out by a bias without end, one that is no number, and ones beside which scores vanish."""
+    x = _logits(300, E, seed=E)
+    for values in ((float("inf"),) * 3, (float("inf"),) * (k + 2), (float("nan"), float("-inf")), (3e38, 3e38, -3e38), (1e6,) * k,
+                   (float("inf"), float("nan"), 3e38, float("-inf"), 1e6)):
+        b = torch.zeros(E, device=DEV)
+        b[torch.randperm(E, generator=torch.Generator().manual_seed(k))[:len(values)].to(DEV)] = torch.tensor(values, device=DEV)
+        ids, _, _ = _compare(x, k, scoring=scoring, bias=b)
+        assert bool((ids.sort(1).values.diff(dim=1) > 0).all())
+
+
+@pytest.mark.parametrize("E,groups", [(64, 8), (512, 8), (96, 3), (40, 5)])
+def test_group_sums_past_single_precision(E, groups):
+    """Two keys of a group add up to more than fp32 holds: the groups are told apart in 64 bits."""
+    g = torch.Generator(device=DEV).manual_seed(E)
+    x = _logits(100, E, seed=3)
+    b = (1.55 + 0.3 * torch.rand(E, generator=g, device=DEV)) * 1e38
+    b[torch.rand(E, generator=g, device=DEV) < 0.3] *= -1.0
+    _compare(x, 6, scoring="sigmoid", bias=b, groups=groups, keep_groups=2)
+
+
 @pytest.mark.parametrize("T,E,k", [(1, 8, 2), (100, 64, 8), (33, 65, 5), (515, 256, 8), (20, 512, 32)])
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("renormalize", [True, False])

@@ -167,6 +167,14 @@ def test_update_by_hand():
     assert R.moment_values(t[3], t[5]).tolist() == pytest.approx([math.sqrt(0.05) * 0.5, 0.0], rel=2.0 ** -4)
 
 
+def test_update_refuses_an_epsilon_that_single_precision_flushes():
+    t = (torch.zeros(8), torch.zeros(8), *F.moments8(8), 0)
+    for eps in (0.0, -1.0, 1e-20, float("nan")):
+        with pytest.raises(ValueError):
+            F.adamw8_many_([t], lr=0.1, eps=eps)
+    F.adamw8_many_([t], lr=0.1, eps=1e-16)
+
+
 def test_update_refuses():
     def lists(n=300):
         return [torch.zeros(n), torch.zeros(n), *F.moments8(n), 0]
