@@ -88,7 +88,8 @@ __device__ unsigned kept_groups(const F* keys, const RouteArgs& a, int lane, F& 
     const F c = __shfl_xor_sync(FULL, best, o), d = __shfl_xor_sync(FULL, second, o);
     merge_top2(best, second, c, d);
   }
-  const F score = size > 1 ? best + second : best;
+  F score = size > 1 ? best + second : best;
+  score = score == score ? score : F(-INFINITY);             // inf - inf
   int ahead = 0;                                 // groups that come before this one
   for (int g = 0; g < a.groups; ++g) {
     const F other = __shfl_sync(FULL, score, g * per);
@@ -102,7 +103,7 @@ __device__ unsigned kept_groups(const F* keys, const RouteArgs& a, int lane, F& 
     worst = w < worst ? w : worst;
     left = l > left ? l : left;
   }
-  gap = worst < F(INFINITY) ? worst - left : F(NAN);         // NaN too where both are -inf: no gap
+  gap = fabs(worst) < F(3e38) ? worst - left : F(NAN);       // near the end of fp32's range a sum says nothing, nor do two of -inf
   unsigned bits = 0;
   for (int g = 0; g < a.groups; ++g) bits |= __shfl_sync(FULL, static_cast<unsigned>(kept), g * per) << g;
   return bits;
@@ -316,7 +317,7 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, bool bias_vect
           second = fmaxf(fmaxf(second, d), fminf(best, c));
           best = fmaxf(best, c);
         }
-        const float score = size > 1 ? best + second : best;
+        const float score = size > 1 ? fmaxf(best + second, -INFINITY) : best;             // NaN of inf - inf: -inf
         const int group = rank / group_lanes;
         int ahead = 0;                           // groups that come before this lane's
         for (int g = 0; g < a.groups; ++g) {
@@ -332,7 +333,7 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, bool bias_vect
           left = fmaxf(left, __shfl_xor_sync(FULL, left, o));
           big = fmaxf(big, __shfl_xor_sync(FULL, big, o));
         }
-        gap = worst < INFINITY ? worst - left : NAN;         // a sum past the type's range says nothing
+        gap = fabsf(worst) < 3e38f ? worst - left : NAN;     // as in kept_groups
         stay = kept ? 1u << group : 0u;          // this lane's own group
       } else {
         float* keys = reinterpret_cast<float*>(keys64);

@@ -316,6 +316,7 @@ def select_experts(logits, k, scoring="softmax", bias=None, groups=1, keep_group
     if groups > 1:
         g = key.view(T, groups, E // groups)
         best = torch.sort(g, dim=-1, descending=True).values[..., :2].sum(-1)
+        best = torch.where(torch.isnan(best), torch.full_like(best, float("-inf")), best)        # inf - inf
         kept = torch.sort(best, dim=-1, descending=True, stable=True).indices[:, :keep_groups]
         drop = torch.ones(T, groups, dtype=torch.bool, device=x.device).scatter_(1, kept, False)
         key = g.masked_fill(drop[..., None], float("-inf")).reshape(T, E)

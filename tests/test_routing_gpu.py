@@ -132,6 +132,19 @@ def test_group_sums_past_single_precision(E, groups):
     b = (1.55 + 0.3 * torch.rand(E, generator=g, device=DEV)) * 1e38
     b[torch.rand(E, generator=g, device=DEV) < 0.3] *= -1.0
     _compare(x, 6, scoring="sigmoid", bias=b, groups=groups, keep_groups=2)
+    _compare(x, 6, scoring="sigmoid", bias=-b.abs(), groups=groups, keep_groups=2)
+
+
+@pytest.mark.parametrize("E,groups", [(16, 8), (64, 8), (96, 3)])
+def test_a_group_with_an_expert_forced_in_and_the_rest_forced_out(E, groups):
+    """inf - inf is no sum: such a group comes last, with those of -inf."""
+    x = _logits(50, E, seed=E)
+    b = torch.zeros(E, device=DEV)
+    b[:E // groups] = float("-inf")
+    b[1] = float("inf")
+    b[-1] = float("inf")
+    for keep in (1, 2, groups):
+        _compare(x, 2, scoring="sigmoid", bias=b, groups=groups, keep_groups=keep)
 
 
 @pytest.mark.parametrize("T,E,k", [(1, 8, 2), (100, 64, 8), (33, 65, 5), (515, 256, 8), (20, 512, 32)])
