@@ -423,9 +423,9 @@ PyObject* preference(PyObject*, PyObject* const* v, Py_ssize_t n) {
       want(none(v[12]));
     }
     const auto options = x.options().dtype(at::kFloat).requires_grad(false);
-    at::Tensor work = empty({6 * R + S + 1 + (logp == nullptr ? R : 0)}, options);
+    at::Tensor work = empty({6 * R + 3 * S + 1 + (logp == nullptr ? R : 0)}, options);
     float* w = static_cast<float*>(work.data_ptr());
-    if (logp == nullptr) logp = w + 6 * R + S + 1;
+    if (logp == nullptr) logp = w + 6 * R + 3 * S + 1;
     launch(grad == nullptr ? PREFERENCE : PREFERENCE_GRAD, ss_preference, x.data_ptr(), f32, pitch(x),
            static_cast<const long long*>(targets.data_ptr()), weights, static_cast<const int*>(cu.data_ptr()), R, V, S / 2, ref,
            static_cast<float>(beta), kind, static_cast<float>(smoothing), v[8] == Py_True, static_cast<float>(number(v[10])), logp, sums,

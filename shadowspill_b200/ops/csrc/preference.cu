@@ -105,12 +105,13 @@ struct PairArgs {
   int kind, average;
 };
 // What the kernels hand on, in one allocation of the caller's. Per row: its weighted log ratio, its weight (0 if nothing is
-// scored), the coefficient, the reference of its exponentials and the reciprocal of their sum. Then the pairs' losses, and
-// counters, zero at the start: rows done of each pair, pairs done.
+// scored), its sequence (-1: none), the reference of its exponentials and the reciprocal of their sum. Per sequence, zero at the
+// start: the coefficient of its rows by their weight. The pairs' losses; and counters, zero at the start: rows done of each pair, pairs
+// done.
 struct Work {
-  double* ratio;
-  float *weight, *coef, *ref, *inv, *pair_loss;
-  int *rows_done, *pairs_done;
+  double *ratio, *slope;
+  float *weight, *ref, *inv, *pair_loss;
+  int *sequence, *rows_done, *pairs_done;
 };
 
 // Exponentials are taken of x - ref, where a row's reference is a multiple of 8 no less than its largest logit: most threads of a row
@@ -200,7 +201,7 @@ __device__ void add_losses(const Rows& rows, const Work& work, float* loss_sum, 
   if (Team<TEAM>::rank() == 0) *loss_sum += static_cast<float>(total);
 }
 
-// The loss of pair p from its rows' log ratios, and its rows' coefficients. By one team, when all rows are done. Sums are held
+// The loss of pair p from its rows' log ratios, and its sequences' slopes. By one team, when all rows are done. Sums are held
 // in 64 bits: they cancel between the two sides.
 template <int TEAM>
 __device__ void finish_pair(int p, const Rows& rows, const PairArgs& a, const Work& work, float* sums, float* loss_sum,
@@ -209,7 +210,7 @@ __device__ void finish_pair(int p, const Rows& rows, const PairArgs& a, const Wo
   const int from = rows.bound(2 * p), between = rows.bound(2 * p + 1), end = rows.bound(2 * p + 2);
   double sum[2] = {0.0, 0.0}, mass[2] = {0.0, 0.0};
   bool any0 = false, any1 = false;
-#pragma unroll 4
+#pragma unroll 8
   for (int r = from + rank; r < end; r += TEAM) {
     const double ratio = __ldcg(work.ratio + r);
     const float w = __ldcg(work.weight + r);
@@ -257,14 +258,10 @@ __device__ void finish_pair(int p, const Rows& rows, const PairArgs& a, const Wo
       slope = 2.0 * gap;
     }
     if (!some) loss = slope = 0.0;
-    if (w < 2) red[0][w] = (w ? mass[1] : mass[0]) != 0.0 ? (w ? slope : -slope) * a.grad_scale / (w ? mass[1] : mass[0]) : 0.0;
-  }
-  Team<TEAM>::sync();
-  const double each[2] = {red[0][0], red[0][1]};
-#pragma unroll 4
-  for (int r = from + rank; r < end; r += TEAM) {
-    const float w = __ldcg(work.weight + r);
-    work.coef[r] = w != 0.f ? static_cast<float>((r >= between ? each[1] : each[0]) * w) : 0.f;
+    if (w < 2) {
+      const double size = w ? mass[1] : mass[0];
+      work.slope[2 * p + w] = size != 0.0 ? (w ? slope : -slope) * a.grad_scale / size : 0.0;
+    }
   }
   if (rows.pairs == 1) {
     if (rank == 0) *loss_sum += static_cast<float>(loss);
@@ -393,11 +390,11 @@ preference_rows_kernel(const L* __restrict__ logits, long long ld, bool aligned,
     work.ratio[row] = 0.0;
   }
   const int before = rows.bounds_up_to(row);
-  const int pair = before > 0 && before <= 2 * rows.pairs ? (before - 1) >> 1 : -1;
+  const int sequence = before > 0 && before <= 2 * rows.pairs ? before - 1 : -1, pair = sequence >> 1;
   bool last = false;
   if (rank == 0) {
     work.weight[row] = scored ? weight : 0.f;
-    work.coef[row] = 0.f;
+    work.sequence[row] = sequence;
     if (pair >= 0) {
       const int all = rows.bound(2 * pair + 2) - rows.bound(2 * pair);
       __threadfence();
@@ -420,7 +417,8 @@ preference_grad_kernel(const L* logits, long long ld, bool aligned, const long l
   constexpr int N = Vec<L>::N, AHEAD = 4;
   const L* x = logits + row * ld;
   L* g = grad + row * ldg;
-  const float coef = work.coef[row];
+  const int sequence = work.sequence[row];
+  const float weight = work.weight[row], coef = sequence >= 0 && weight != 0.f ? static_cast<float>(work.slope[sequence] * weight) : 0.f;
   const int pieces = V / N;
   if (coef == 0.f) {
     const float zero[N] = {};
@@ -480,7 +478,7 @@ int preference(const L* logits, long long ld, const Rows& rows, const PairArgs& 
                float* loss_sum, L* grad, long long ldg, cudaStream_t s) {
   auto aligned16 = [&](const L* x, long long pitch) { return reinterpret_cast<uintptr_t>(x) % 16 == 0 && pitch % Vec<L>::N == 0; };
   const bool aligned = aligned16(logits, ld) && (grad == nullptr || aligned16(grad, ldg));
-  const cudaError_t e = cudaMemsetAsync(work.rows_done, 0, sizeof(int) * (rows.pairs + 1ll), s);
+  const cudaError_t e = cudaMemsetAsync(work.slope, 0, 8ll * 2 * rows.pairs + sizeof(int) * (rows.pairs + 1ll), s);
   if (e != cudaSuccess) return (int)e;
   const int pieces = rows.V / Vec<L>::N;
   auto statistics = [&](auto team) {
@@ -494,8 +492,8 @@ int preference(const L* logits, long long ld, const Rows& rows, const PairArgs& 
                    aligned, rows.targets, work, rows.R, rows.V, grad, ldg);
   };
   // A row's team grows until the block has threads enough for the GPU and no thread has less than four pieces. Whole calls, us, by team of 32 /
-  // 128 / 256 / 512 / 1024 for the statistics: 8,000 rows of 2,500 words 50 / 60 / 87 / 135 / 268; 1,000 of 5,000 30 / 27 / 30 / 35 / 50;
-  // 4,096 of 128,256 484 / 430 / 429 / 451 / 529; 200 of 151,936 154 / 72 / 56 / 53 / 50.
+  // 128 / 256 / 512 / 1024, without the gradient: 8,000 rows of 2,500 words 40 / 45 / 63 / 128 / 340; 1,000 of 5,000 35 / 16 / 18 / 27 / 51;
+  // 4,096 of 128,256 - / 148 / 150 / 184 / 295; 200 of 151,936 - / 47 / 35 / 29 / 29.
   int team = pieces <= 1024 ? 32 : 128;
   while (team < 1024 && static_cast<long long>(rows.R) * team < 148 * 1024) {
     const int next = team == 32 ? 128 : 2 * team;
@@ -523,7 +521,7 @@ int preference(const L* logits, long long ld, const Rows& rows, const PairArgs& 
 extern "C" {
 using namespace ss;
 
-// work: 6 R + 2 pairs + 1 words on a boundary of 8 bytes. logp: R words. grad null: the loss alone.
+// work: 6 R + 6 pairs + 1 words on a boundary of 8 bytes. logp: R words. grad null: the loss alone.
 int ss_preference(const void* logits, int fp32_logits, long long ld, const long long* targets, const float* weights,
                   const int* cu_seqlens, int R, int V, int pairs, const float* ref_logp, float beta, int kind, float smoothing,
                   int average, float grad_scale, float* logp, float* sums, float* loss_sum, void* grad, long long ldg, void* work,
@@ -531,9 +529,11 @@ int ss_preference(const void* logits, int fp32_logits, long long ld, const long 
   if (R < 0 || R > 0x7fff0000 || V < 1 || pairs < 0 || pairs > 0x3fffffff || kind < 0 || kind > 2 || ld < V || (grad != nullptr && ldg < V)) return -2;
   const Rows rows{targets, weights, ref_logp, cu_seqlens, R, V, pairs};
   const PairArgs a{beta, smoothing, grad_scale, kind, average};
-  const long long n = R;
-  float* w = (float*)work + 2 * n;
-  const Work handed{(double*)work, w, w + n, w + 2 * n, w + 3 * n, w + 4 * n, (int*)(w + 4 * n + pairs), (int*)(w + 4 * n + 2 * pairs)};
+  const long long n = R, p = pairs;
+  double* d = (double*)work;                     // ratio, slope; then the counters, which are cleared with the slopes; then the rest
+  int* c = (int*)(d + n + 2 * p);
+  float* w = (float*)(c + p + 1);
+  const Work handed{d, d + n, w, w + n, w + 2 * n, w + 4 * n, (int*)(w + 3 * n), c, c + p};
   cudaStream_t s = (cudaStream_t)stream;
   if (fp32_logits) return preference((const float*)logits, ld, rows, a, handed, logp, sums, loss_sum, (float*)grad, ldg, s);
   return preference((const bf16*)logits, ld, rows, a, handed, logp, sums, loss_sum, (bf16*)grad, ldg, s);

@@ -535,7 +535,7 @@ def preference_(logits, targets, weights, cu_seqlens, loss_sum, *, beta=0.1, kin
     if R > 1 and (logits.stride(0) < V or (out is not None and out.stride(0) < V)):
         raise ValueError("rows of logits and of their gradient do not overlap")
     with _device_of(logits):
-        work = torch.empty(6 * R + S + 1, dtype=torch.float32, device=logits.device)
+        work = torch.empty(6 * R + 3 * S + 1, dtype=torch.float32, device=logits.device)
         lp = torch.empty(R, dtype=torch.float32, device=logits.device) if logp is None else logp
         _lib.check(_lib.lib().ss_preference(
             logits.data_ptr(), int(logits.dtype == torch.float32), max(logits.stride(0), V), targets.data_ptr(), _ptr(weights),
