@@ -6,8 +6,10 @@
 //   dL/dx_r = coef_r (softmax(x_r) - onehot(t_r)),  coef_r = -+ beta f'(z_p) w_r [/ sum of w_r]
 // with f = -(1 - e) log sigma(z) - e log sigma(-z), max(0, 1 - z) or (z / beta - 1 / (2 beta))^2.
 //
-// A row's gradient needs every row of its pair first, so the block is read twice: once for the rows' statistics, whose last
-// row of a pair forms the pair's loss and coefficients, once for the gradient.
+// A row's gradient needs every row of its pair first, so the block is read twice: once for the rows' statistics, where the last row of a
+// pair to be done forms the pair's loss and slopes, once for the gradient. Both are bound by memory where the block is large: 4,096 rows of
+// 128,256 bf16 words, 70 % of them scored, take 418 us of which 388 are two reads and a write at the copy rate; 24 rows of 4,096
+// are three launches, 15 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <float.h>
@@ -58,21 +60,34 @@ template <> struct Vec<float> {
   __device__ static float put(float v) { return v; }
 };
 
-// The c-th piece of a row that may start anywhere: the same elements to a thread, hence the same bits, as of aligned rows.
+// The c-th of a row's `pieces` where the row starts anywhere: the same elements to a thread, hence the same bits, as of aligned rows. The two
+// aligned 16 bytes that hold it are read and moved together; the first and last piece go by element, so that nothing
+// outside the row is read. (4,096 rows of 50,257 words, without the gradient: 149 us by elements throughout, 100 for 50,256.)
 template <class L>
-__device__ __forceinline__ void load_piece(const L* x, int c, bool aligned, float (&f)[Vec<L>::N]) {
-  if (aligned) return Vec<L>::load(reinterpret_cast<const uint4*>(x)[c], f);
+__device__ __forceinline__ void load_piece(const L* x, int c, int pieces, float (&f)[Vec<L>::N]) {
+  const L* at = x + static_cast<long long>(c) * Vec<L>::N;
+  if (c == 0 || c == pieces - 1) {
 #pragma unroll
-  for (int e = 0; e < Vec<L>::N; ++e) f[e] = Vec<L>::get(x[c * Vec<L>::N + e]);
-}
-template <class L>
-__device__ __forceinline__ void store_piece(L* x, int c, bool aligned, const float (&f)[Vec<L>::N]) {
-  if (aligned) {
-    reinterpret_cast<uint4*>(x)[c] = Vec<L>::store(f);
+    for (int e = 0; e < Vec<L>::N; ++e) f[e] = Vec<L>::get(at[e]);
     return;
   }
+  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(x) & 15);
+  const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(at) - off);
+  const uint4 u = q[0], v = q[1];
+  uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int e = 0; e < Vec<L>::N; ++e) x[c * Vec<L>::N + e] = Vec<L>::put(f[e]);
+  for (int i = 0; i < 6; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = off & 2 ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+  Vec<L>::load(make_uint4(w[0], w[1], w[2], w[3]), f);
+}
+
+template <class L>
+__device__ __forceinline__ void store_elements(L* to, const float (&f)[Vec<L>::N]) {
+#pragma unroll
+  for (int e = 0; e < Vec<L>::N; ++e) to[e] = Vec<L>::put(f[e]);
 }
 
 struct Rows {
@@ -295,7 +310,9 @@ __device__ void finish_empty(const Rows& rows, const Work& work, float* sums, fl
   if (Team<TEAM>::any(last)) add_losses<TEAM>(rows, work, loss_sum, red);
 }
 
-// A team per row, and one more for the pairs without rows.
+// A team per row, and one more for the pairs without rows. 735 MB of rows of 128,256 words: 133 us, 5.5 TB/s, the units of ex2 busy in 74 % of
+// the cycles and half the issue slots; without exponentials it would be 122. Loads through a ring in shared memory, a part
+// of the exponentials by multiply-adds and blocks that stay while one warp finishes rows for the others were no faster.
 template <class L, int TEAM>
 __global__ void __launch_bounds__(Team<TEAM>::BLOCK)
 preference_rows_kernel(const L* __restrict__ logits, long long ld, bool aligned, Rows rows, PairArgs a, Work work,
@@ -337,7 +354,7 @@ preference_rows_kernel(const L* __restrict__ logits, long long ld, bool aligned,
     }
     for (; c < pieces; c += TEAM) {
       float f[N];
-      load_piece(x, c, aligned, f);
+      load_piece(x, c, pieces, f);
       part.add(f);
     }
     for (c = pieces * N + rank; c < rows.V; c += TEAM) {
@@ -406,11 +423,14 @@ preference_rows_kernel(const L* __restrict__ logits, long long ld, bool aligned,
   finish_pair<TEAM>(pair, rows, a, work, sums, loss_sum, red);
 }
 
-// From the last row to the first: the rows read last are still in the L2.
+// From the last row to the first: the rows read last are still in the L2. Nothing is summed here, so a thread may have any elements: the pieces
+// on the row's 16-byte boundaries and the few elements before and behind them, stored by element where the
+// gradient's boundaries lie elsewhere. Bound by memory: 1.05 GB written and 0.74 read in 272 us, 6.5 TB/s (4,096 rows of 128,256 words, 70 % scored).
+// 4,096 rows of 50,257 words, whole calls: 271 us, by element from the row's start 616; of 50,256 words 229. (The choice at the
+// store stays in the loop: without it a thread's four stores leave together, 243 us.)
 template <class L, int TEAM>
 __global__ void __launch_bounds__(Team<TEAM>::BLOCK)
-preference_grad_kernel(const L* logits, long long ld, bool aligned, const long long* targets, Work work, int R, int V,
-                       L* grad, long long ldg) {
+preference_grad_kernel(const L* logits, long long ld, const long long* targets, Work work, int R, int V, L* grad, long long ldg) {
   chain_wait();
   const int row = R - 1 - Team<TEAM>::row(), rank = Team<TEAM>::rank();
   if (row < 0) return;
@@ -419,11 +439,19 @@ preference_grad_kernel(const L* logits, long long ld, bool aligned, const long l
   L* g = grad + row * ldg;
   const int sequence = work.sequence[row];
   const float weight = work.weight[row], coef = sequence >= 0 && weight != 0.f ? static_cast<float>(work.slope[sequence] * weight) : 0.f;
-  const int pieces = V / N;
+  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(x) & 15);
+  const bool together = off == static_cast<int>(reinterpret_cast<uintptr_t>(g) & 15);
+  const int head = min(static_cast<int>(((16 - off) & 15) / sizeof(L)), V), pieces = (V - head) / N;
+  const int rest = V - pieces * N;
+  auto single = [&](int i) { return i < head ? i : i + pieces * N; };          // the i-th element outside the pieces
+  uint4* gv = reinterpret_cast<uint4*>(g + head);
   if (coef == 0.f) {
     const float zero[N] = {};
-    for (int c = rank; c < pieces; c += TEAM) store_piece(g, c, aligned, zero);
-    for (int c = pieces * N + rank; c < V; c += TEAM) g[c] = Vec<L>::put(0.f);
+    for (int c = rank; c < pieces; c += TEAM) {
+      if (together) gv[c] = make_uint4(0, 0, 0, 0);
+      else store_elements(g + head + c * N, zero);
+    }
+    for (int i = rank; i < rest; i += TEAM) g[single(i)] = Vec<L>::put(0.f);
     return;
   }
   const float ref = work.ref[row], inv = work.inv[row], each = coef * fabsf(inv);
@@ -433,7 +461,10 @@ preference_grad_kernel(const L* logits, long long ld, bool aligned, const long l
       g[c] = Vec<L>::put(each * expf(Vec<L>::get(x[c]) - ref) - (c == target ? coef : 0.f));
     return;
   }
-  auto piece = [&](float (&f)[N], int c) {
+  const int among = target - head, target_piece = among >= 0 ? among / N : -1;         // from the first piece on; -1: in none
+  auto piece = [&](const uint4& u, int c) {
+    float f[N];
+    Vec<L>::load(u, f);
 #pragma unroll
     for (int e = 0; e < N; e += 2) {
       const float2 y = exponents(f[e], f[e + 1], -ref);
@@ -441,43 +472,34 @@ preference_grad_kernel(const L* logits, long long ld, bool aligned, const long l
       f[e] = v.x;
       f[e + 1] = v.y;
     }
-    if (c == target / N) {
+    if (c == target_piece) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) f[e] -= e == target % N ? coef : 0.f;
+      for (int e = 0; e < N; ++e) f[e] = __fadd_rn(f[e], e == among % N ? -coef : 0.f);
     }
-    store_piece(g, c, aligned, f);
+    if (together) gv[c] = Vec<L>::store(f);
+    else store_elements(g + head + c * N, f);
   };
+  const uint4* xv = reinterpret_cast<const uint4*>(x + head);
   int c = rank;
-  if (aligned) {
-    const uint4* xv = reinterpret_cast<const uint4*>(x);
-    for (; c + (AHEAD - 1) * TEAM < pieces; c += AHEAD * TEAM) {
-      uint4 u[AHEAD];
+  for (; c + (AHEAD - 1) * TEAM < pieces; c += AHEAD * TEAM) {
+    uint4 u[AHEAD];
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) u[i] = xv[c + i * TEAM];
+    for (int i = 0; i < AHEAD; ++i) u[i] = xv[c + i * TEAM];
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        float f[N];
-        Vec<L>::load(u[i], f);
-        piece(f, c + i * TEAM);
-      }
-    }
+    for (int i = 0; i < AHEAD; ++i) piece(u[i], c + i * TEAM);
   }
-  for (; c < pieces; c += TEAM) {
-    float f[N];
-    load_piece(x, c, aligned, f);
-    piece(f, c);
-  }
-  for (c = pieces * N + rank; c < V; c += TEAM) {
-    const float2 y = exponents(Vec<L>::get(x[c]), 0.f, -ref);
-    g[c] = Vec<L>::put(each * ex2(y.x) - (c == target ? coef : 0.f));
+  for (; c < pieces; c += TEAM) piece(xv[c], c);
+  for (int i = rank; i < rest; i += TEAM) {
+    const int at = single(i);
+    const float2 y = exponents(Vec<L>::get(x[at]), 0.f, -ref);
+    g[at] = Vec<L>::put(__fadd_rn(__fmul_rn(ex2(y.x), each), at == target ? -coef : 0.f));     // as in a piece
   }
 }
 
 template <class L>
 int preference(const L* logits, long long ld, const Rows& rows, const PairArgs& a, const Work& work, float* logp, float* sums,
                float* loss_sum, L* grad, long long ldg, cudaStream_t s) {
-  auto aligned16 = [&](const L* x, long long pitch) { return reinterpret_cast<uintptr_t>(x) % 16 == 0 && pitch % Vec<L>::N == 0; };
-  const bool aligned = aligned16(logits, ld) && (grad == nullptr || aligned16(grad, ldg));
+  const bool aligned = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && ld % Vec<L>::N == 0;
   const cudaError_t e = cudaMemsetAsync(work.slope, 0, 8ll * 2 * rows.pairs + sizeof(int) * (rows.pairs + 1ll), s);
   if (e != cudaSuccess) return (int)e;
   const int pieces = rows.V / Vec<L>::N;
@@ -489,7 +511,7 @@ int preference(const L* logits, long long ld, const Rows& rows, const PairArgs& 
   auto gradient = [&](auto team) {
     using T = Team<decltype(team)::value>;
     launch_chained(preference_grad_kernel<L, decltype(team)::value>, (rows.R + T::ROWS - 1) / T::ROWS, T::BLOCK, 0, s, logits, ld,
-                   aligned, rows.targets, work, rows.R, rows.V, grad, ldg);
+                   rows.targets, work, rows.R, rows.V, grad, ldg);
   };
   // A row's team grows until the block has threads enough for the GPU and no thread has less than four pieces. Whole calls, us, by team of 32 /
   // 128 / 256 / 512 / 1024, without the gradient: 8,000 rows of 2,500 words 40 / 45 / 63 / 128 / 340; 1,000 of 5,000 35 / 16 / 18 / 27 / 51;

@@ -175,6 +175,31 @@ def test_strided_and_unaligned_logits(dtype, wide, skip):
     assert float(a) == pytest.approx(float(b), rel=1e-5)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [3, 9, 17, 130, 1001, 4110, 50257])
+def test_bits_do_not_depend_on_where_rows_lie(V, dtype):
+    x, t, w, cu, ref = _case(V, [0, 9, 20], 21, dtype, seed=V, masked=0.1)
+    t[:8] = torch.tensor([0, V - 1, min(7, V - 1), min(8, V - 1), max(V - 2, 0), V // 2, min(1, V - 1), max(V - 9, 0)], device=DEV)
+    rows = []
+    pitch = -(-V // 8) * 8
+    for skip in range(8):
+        buffer = torch.full((21 * pitch + 24,), 5.0, dtype=dtype, device=DEV)
+        for wide in (V, pitch):
+            at = torch.as_strided(buffer, (21, V), (wide, 1), skip)
+            at.copy_(x)
+            loss, logp = torch.zeros(1, device=DEV), torch.empty(21, device=DEV)
+            other = torch.empty(21, V, dtype=dtype, device=DEV)
+            F.preference_(at, t, w, cu, loss, ref_logp=ref, logp=logp, grad=other)
+            F.preference_(at, t, w, cu, loss, ref_logp=ref, logp=logp)
+            rows.append((loss, logp, at.clone(), other))
+            around = torch.ones_like(buffer, dtype=torch.bool)
+            torch.as_strided(around, (21, V), (wide, 1), skip).fill_(False)
+            assert bool((buffer[around] == 5.0).all())            # what lies between and around the rows is left as it was
+            buffer.fill_(5.0)
+    for got in rows:
+        assert all(torch.equal(a, b) for a, b in zip(got, rows[0])) and torch.equal(got[2], got[3])
+
+
 def test_saturated_margins_and_hinge_without_loss():
     x, t, w, cu, _ = _case(600, [0, 30, 60, 90, 120], 120, torch.float32, seed=6, masked=0.0)
     for far in (-60.0, 60.0):                                    # the reference far off: z near +-100
