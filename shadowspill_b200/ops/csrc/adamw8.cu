@@ -19,6 +19,7 @@
 #include <math.h>
 #include <stdint.h>
 
+#include "chained_launch.cuh"
 #include "launchers.h"
 
 namespace ss {
@@ -254,6 +255,8 @@ __global__ void __launch_bounds__(A8_THREADS, 3)
 adamw8_kernel(const __grid_constant__ Table8 tab, Args8 a) {
   using Ring = Ring8<P, G>;
   __shared__ __align__(16) unsigned char ring[A8_WARPS][Ring::STAGES][Ring::STAGE];
+  chain_wait();
+  chain_release();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int lo = 0, hi = tab.count - 1;                // the last tensor that starts at or before this CTA
   while (lo < hi) {
@@ -372,7 +375,7 @@ adamw8_kernel(const __grid_constant__ Table8 tab, Args8 a) {
 template <class P, class G>
 int launch8(const Table8& tab, const Args8& a, int runs, int sr_param, int sr_state, cudaStream_t s) {
   auto go = [&](auto kern) {
-    kern<<<runs, A8_THREADS, 0, s>>>(tab, a);
+    launch_chained(kern, runs, A8_THREADS, 0, s, tab, a);
     return (int)cudaGetLastError();
   };
   if (sizeof(P) == 2 && sr_param)

@@ -310,21 +310,30 @@ __device__ void finish_empty(const Rows& rows, const Work& work, float* sums, fl
   if (Team<TEAM>::any(last)) add_losses<TEAM>(rows, work, loss_sum, red);
 }
 
+__global__ void clear_counters_kernel(int* words, int n) {
+  chain_wait();
+  chain_release();
+  for (int i = threadIdx.x; i < n; i += blockDim.x) words[i] = 0;
+}
+
 // A team per row, and one more for the pairs without rows. 735 MB of rows of 128,256 words: 133 us, 5.5 TB/s, the units of ex2 busy in 74 % of
 // the cycles and half the issue slots; without exponentials it would be 122. Loads through a ring in shared memory, a part
 // of the exponentials by multiply-adds and blocks that stay while one warp finishes rows for the others were no faster.
 template <class L, int TEAM>
 __global__ void __launch_bounds__(Team<TEAM>::BLOCK)
-preference_rows_kernel(const L* __restrict__ logits, long long ld, bool aligned, Rows rows, PairArgs a, Work work,
-                       float* __restrict__ logp, float* __restrict__ sums, float* __restrict__ loss_sum) {
+preference_rows_kernel(const L* logits, long long ld, bool aligned, Rows rows, PairArgs a, Work work, float* logp, float* sums,
+                       float* loss_sum) {
   constexpr int WARPS = TEAM / 32;
   __shared__ double red_of[Team<TEAM>::ROWS][4][WARPS];
   __shared__ double parts[WARPS];                // of teams of several warps
   __shared__ float refs[WARPS], tops[WARPS];
   const int rank = Team<TEAM>::rank(), row = Team<TEAM>::row();
   double (*red)[WARPS] = red_of[threadIdx.x / TEAM];
+  // This kernel starts beside the one that clears its counters, which has waited for all work before; the
+  // counters alone have to be waited for.
   if (row > rows.R) return;
   if (row == rows.R) {
+    chain_wait();
     finish_empty<TEAM>(rows, work, sums, loss_sum, red[0]);
     return;
   }
@@ -407,6 +416,7 @@ preference_rows_kernel(const L* __restrict__ logits, long long ld, bool aligned,
     work.ratio[row] = 0.0;
   }
   const int before = rows.bounds_up_to(row);
+  chain_wait();
   const int sequence = before > 0 && before <= 2 * rows.pairs ? before - 1 : -1, pair = sequence >> 1;
   bool last = false;
   if (rank == 0) {
@@ -500,13 +510,12 @@ template <class L>
 int preference(const L* logits, long long ld, const Rows& rows, const PairArgs& a, const Work& work, float* logp, float* sums,
                float* loss_sum, L* grad, long long ldg, cudaStream_t s) {
   const bool aligned = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && ld % Vec<L>::N == 0;
-  const cudaError_t e = cudaMemsetAsync(work.slope, 0, 8ll * 2 * rows.pairs + sizeof(int) * (rows.pairs + 1ll), s);
-  if (e != cudaSuccess) return (int)e;
+  launch_chained(clear_counters_kernel, 1, rows.pairs < 64 ? 128 : 1024, 0, s, reinterpret_cast<int*>(work.slope), 5 * rows.pairs + 1);
   const int pieces = rows.V / Vec<L>::N;
   auto statistics = [&](auto team) {
     using T = Team<decltype(team)::value>;
-    preference_rows_kernel<L, decltype(team)::value><<<rows.R / T::ROWS + 1, T::BLOCK, 0, s>>>(
-        logits, ld, aligned, rows, a, work, logp, sums, loss_sum);
+    launch_chained(preference_rows_kernel<L, decltype(team)::value>, rows.R / T::ROWS + 1, T::BLOCK, 0, s, logits, ld, aligned, rows, a, work,
+                   logp, sums, loss_sum);
   };
   auto gradient = [&](auto team) {
     using T = Team<decltype(team)::value>;
@@ -548,7 +557,7 @@ int ss_preference(const void* logits, int fp32_logits, long long ld, const long 
                   const int* cu_seqlens, int R, int V, int pairs, const float* ref_logp, float beta, int kind, float smoothing,
                   int average, float grad_scale, float* logp, float* sums, float* loss_sum, void* grad, long long ldg, void* work,
                   void* stream) {
-  if (R < 0 || R > 0x7fff0000 || V < 1 || pairs < 0 || pairs > 0x3fffffff || kind < 0 || kind > 2 || ld < V || (grad != nullptr && ldg < V)) return -2;
+  if (R < 0 || R > 0x7fff0000 || V < 1 || pairs < 0 || pairs > 0xfffffff || kind < 0 || kind > 2 || ld < V || (grad != nullptr && ldg < V)) return -2;
   const Rows rows{targets, weights, ref_logp, cu_seqlens, R, V, pairs};
   const PairArgs a{beta, smoothing, grad_scale, kind, average};
   const long long n = R, p = pairs;

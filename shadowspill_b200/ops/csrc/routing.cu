@@ -16,6 +16,7 @@
 
 #include <type_traits>
 
+#include "chained_launch.cuh"
 #include "launchers.h"
 
 namespace ss {
@@ -226,8 +227,11 @@ __device__ __forceinline__ void load_row(const L* row, int first, int E, bool ve
 constexpr int rt_resident(int per) { return per == 16 ? 7 : 8; }     // blocks that an SM's registers hold
 template <int LANES, int PER, bool LOGITS, class L>
 __global__ void __launch_bounds__(RT_THREADS, rt_resident(PER))
-select_experts_kernel(const L* __restrict__ logits, bool vectors, bool bias_vectors, RouteArgs a, int* __restrict__ ids, float* __restrict__ weights,
-                      int* __restrict__ counts) {
+select_experts_kernel(const L* logits, bool vectors, bool bias_vectors, RouteArgs a, int* ids, float* weights, int* counts) {
+  // Several blocks count behind the kernel that clears the counts, which lets this one start beside it, after its own wait for
+  // all work before: what it waits for itself is the cleared counts alone, at the end.
+  const bool alone = gridDim.x == 1;
+  if (alone) chain_wait();
   constexpr int TOKENS = 32 / LANES;             // of a warp
   __shared__ int hist[RT_MAX_E];
   __shared__ unsigned char group_of[RT_MAX_E];
@@ -524,11 +528,19 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, bool bias_vect
       atomicAdd(&hist[mine], 1);
     }
   }
+  chain_release();
+  if (!alone) chain_wait();
   __syncthreads();
   for (int e = threadIdx.x; e < a.E; e += RT_THREADS) {
-    if (gridDim.x == 1) counts[e] = hist[e];
+    if (alone) counts[e] = hist[e];
     else if (hist[e]) atomicAdd(counts + e, hist[e]);
   }
+}
+
+__global__ void clear_counts_kernel(int* counts, int E) {
+  chain_wait();
+  chain_release();
+  for (int e = threadIdx.x; e < E; e += blockDim.x) counts[e] = 0;
 }
 
 // With c_j the picked scores, S their sum: dc_j = scale / S (dw_j - sum_i dw_i c_i / S) or scale dw_j, and
@@ -537,8 +549,9 @@ select_experts_kernel(const L* __restrict__ logits, bool vectors, bool bias_vect
 // 8,192 x 64 in 4.4, of which a launch is half.
 template <class L>
 __global__ void __launch_bounds__(RT_THREADS)
-select_experts_bwd_kernel(const L* __restrict__ logits, RouteArgs a, const int* __restrict__ ids,
-                          const float* __restrict__ dweights, L* __restrict__ dlogits) {
+select_experts_bwd_kernel(const L* logits, RouteArgs a, const int* ids, const float* dweights, L* dlogits) {
+  chain_wait();
+  chain_release();
   const int lane = threadIdx.x & 31;
   for (int t = blockIdx.x * RT_WARPS + (threadIdx.x >> 5); t < a.T; t += gridDim.x * RT_WARPS) {
     const L* row = logits + static_cast<long long>(t) * a.ld;
@@ -610,13 +623,11 @@ int ss_select_experts(const void* logits, int bf16_logits, long long ld, const f
   const int lanes = halves ? 16 : 32, per_block = RT_WARPS * (halves ? 2 : 1);
   const int per = (E + lanes - 1) / lanes, most = 148 * rt_resident(per <= 8 ? 8 : 16);
   const int blocks = (T + per_block - 1) / per_block, grid = blocks < 1 ? 1 : blocks < most ? blocks : most;
-  if (grid > 1) {                                // a single block writes the counts whole
-    const cudaError_t e = cudaMemsetAsync(counts, 0, sizeof(int) * E, s);
-    if (e != cudaSuccess) return (int)e;
-  }
+  if (grid > 1) launch_chained(clear_counts_kernel, 1, 128, 0, s, counts, E);          // a single block writes the counts whole
   auto go = [&](auto kern, auto* x) {
     const bool vectors = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld * sizeof(*x) % 16 == 0;
-    kern<<<grid, RT_THREADS, plain ? 0 : sizeof(double) * E * RT_WARPS, s>>>(x, vectors, reinterpret_cast<uintptr_t>(bias) % 16 == 0, a, ids, weights, counts);
+    launch_chained(kern, grid, RT_THREADS, plain ? 0 : sizeof(double) * E * RT_WARPS, s, x, vectors, reinterpret_cast<uintptr_t>(bias) % 16 == 0,
+                   a, ids, weights, counts);
     return (int)cudaGetLastError();
   };
   auto by_mode = [&](auto* x, auto logits_only) {
@@ -644,12 +655,12 @@ int ss_select_experts_bwd(const void* logits, int bf16_logits, long long ld, con
   if (!fits(a)) return -2;
   if (T == 0) return 0;
   const int blocks = (T + RT_WARPS - 1) / RT_WARPS, grid = blocks < 148 * 16 ? blocks : 148 * 16;
-  if (bf16_logits)
-    select_experts_bwd_kernel<<<grid, RT_THREADS, 0, (cudaStream_t)stream>>>((const __nv_bfloat16*)logits, a, ids, dweights,
-                                                                             (__nv_bfloat16*)dlogits);
-  else
-    select_experts_bwd_kernel<<<grid, RT_THREADS, 0, (cudaStream_t)stream>>>((const float*)logits, a, ids, dweights,
-                                                                             (float*)dlogits);
+  auto go = [&](auto kern, auto* x) {
+    launch_chained(kern, grid, RT_THREADS, 0, (cudaStream_t)stream, x, a, ids, dweights, const_cast<std::remove_const_t<std::remove_pointer_t<decltype(x)>>*>(
+        reinterpret_cast<decltype(x)>(dlogits)));
+  };
+  if (bf16_logits) go(select_experts_bwd_kernel<__nv_bfloat16>, (const __nv_bfloat16*)logits);
+  else go(select_experts_bwd_kernel<float>, (const float*)logits);
   return (int)cudaGetLastError();
 }
 }  // extern "C"
