@@ -510,7 +510,10 @@ template <class L>
 int preference(const L* logits, long long ld, const Rows& rows, const PairArgs& a, const Work& work, float* logp, float* sums,
                float* loss_sum, L* grad, long long ldg, cudaStream_t s) {
   const bool aligned = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && ld % Vec<L>::N == 0;
-  launch_chained(clear_counters_kernel, 1, rows.pairs < 64 ? 128 : 1024, 0, s, reinterpret_cast<int*>(work.slope), 5 * rows.pairs + 1);
+  // The rows kernel starts beside the kernel that clears its counters. Behind short ones the host is waited for, and a memset is
+  // less of its time than a third kernel: 24 rows of 4,096 words 15.0 us with it and 15.7 with a kernel, 333 rows of 32,003 36 and 33.5.
+  if (static_cast<long long>(rows.R) * rows.V < 1 << 21) cudaMemsetAsync(work.slope, 0, sizeof(int) * (5ll * rows.pairs + 1), s);
+  else launch_chained(clear_counters_kernel, 1, rows.pairs < 64 ? 128 : 1024, 0, s, reinterpret_cast<int*>(work.slope), 5 * rows.pairs + 1);
   const int pieces = rows.V / Vec<L>::N;
   auto statistics = [&](auto team) {
     using T = Team<decltype(team)::value>;
