@@ -134,7 +134,7 @@ template <> struct Piece8<float> {
   float4 a, b;
   __device__ __forceinline__ void load(const uint4* x) {
     a = *reinterpret_cast<const float4*>(x);
-    b = *reinterpret_cast<const float4*>(x + 32);
+    b = *reinterpret_cast<const float4*>(x + 1);
   }
   __device__ __forceinline__ void set(int e, float x) { (e < 4 ? reinterpret_cast<float*>(&a) : reinterpret_cast<float*>(&b))[e & 3] = x; }
   __device__ __forceinline__ void get(Eight& f) const {
@@ -243,8 +243,8 @@ __device__ __forceinline__ void copy8(const void* to, const void* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
 }
 
-// A warp walks `run` blocks, a CTA's eight warps side by side. Blocks to come are on their way in shared memory, where a lane reads
-// only what it asked for itself, so nothing but its own copies is waited for. (With the next block in registers instead the
+// A warp walks `run` blocks, a CTA's eight warps side by side. Blocks to come are on their way in shared memory, copied and stored by
+// whole sectors: eight fp32 elements of a lane are 32 bytes, which two instructions of 16 would each ask for by halves. (With the next block in registers instead the
 // compiler moves the loads down to their use for want of registers: 218 M elements 668 us.)
 template <class P, class G> struct Ring8 {
   static constexpr int P16 = sizeof(P) / 2, G16 = sizeof(G) / 2;       // 16-byte pieces of a lane
@@ -279,13 +279,14 @@ adamw8_kernel(const __grid_constant__ Table8 tab, Args8 a) {
   auto fetch = [&](int i) {
     if (i < full) {
       const long long e0 = (first + static_cast<long long>(i) * A8_WARPS) * A8_BLOCK + lane * 8;
-      uint4* q = reinterpret_cast<uint4*>(ring[warp][i % Ring::STAGES]) + lane;
+      uint4* q = reinterpret_cast<uint4*>(ring[warp][i % Ring::STAGES]);
+      const long long block = e0 - lane * 8;
 #pragma unroll
-      for (int k = 0; k < Ring::P16; ++k) copy16(q + 32 * k, reinterpret_cast<const uint4*>(p + e0) + k);
+      for (int k = 0; k < Ring::P16; ++k) copy16(q + lane + 32 * k, reinterpret_cast<const uint4*>(p + block) + lane + 32 * k);
       q += 32 * Ring::P16;
 #pragma unroll
-      for (int k = 0; k < Ring::G16; ++k) copy16(q + 32 * k, reinterpret_cast<const uint4*>(g + e0) + k);
-      uint2* c = reinterpret_cast<uint2*>(q - lane + 32 * Ring::G16) + lane;
+      for (int k = 0; k < Ring::G16; ++k) copy16(q + lane + 32 * k, reinterpret_cast<const uint4*>(g + block) + lane + 32 * k);
+      uint2* c = reinterpret_cast<uint2*>(q + 32 * Ring::G16) + lane;
       copy8(c, t.m + e0);
       copy8(c + 32, t.r + e0);
     }
@@ -299,11 +300,12 @@ adamw8_kernel(const __grid_constant__ Table8 tab, Args8 a) {
   for (; i < full; ++i) {
     asm volatile("cp.async.wait_group %0;" ::"n"(Ring::STAGES - 2) : "memory");
     const long long e0 = (first + static_cast<long long>(i) * A8_WARPS) * A8_BLOCK + lane * 8;
-    const uint4* q = reinterpret_cast<const uint4*>(ring[warp][i % Ring::STAGES]) + lane;
-    x.p.load(q);
+    __syncwarp();                                // copies of other lanes, where a lane's eight elements are two pieces
+    const uint4* q = reinterpret_cast<const uint4*>(ring[warp][i % Ring::STAGES]);
+    x.p.load(q + lane * Ring::P16);
     q += 32 * Ring::P16;
-    x.g.load(q);
-    const uint2* c = reinterpret_cast<const uint2*>(q - lane + 32 * Ring::G16) + lane;
+    x.g.load(q + lane * Ring::G16);
+    const uint2* c = reinterpret_cast<const uint2*>(q + 32 * Ring::G16) + lane;
     x.m = c[0];
     x.r = c[32];
     x.m_exp = __shfl_sync(0xffffffffu, m_exp, i);
@@ -311,9 +313,20 @@ adamw8_kernel(const __grid_constant__ Table8 tab, Args8 a) {
     fetch(i + Ring::STAGES - 1);                 // into the stage of the block before this one
     update8<SR_PARAM, SR_STATE>(x, a, t.offset + static_cast<unsigned long long>(e0), out, random);
     if (sizeof(P) == 4) {
-      float4* to4 = reinterpret_cast<float4*>(p + e0);
-      to4[0] = make_float4(out.v[0].x, out.v[0].y, out.v[1].x, out.v[1].y);
-      to4[1] = make_float4(out.v[2].x, out.v[2].y, out.v[3].x, out.v[3].y);
+      // two lanes write the halves of the even one's eight elements, then those of the odd one's: whole sectors
+      const bool odd = lane & 1;
+      float2 own[2], other[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float2 gives = odd ? out.v[k] : out.v[2 + k];
+        own[k] = odd ? out.v[2 + k] : out.v[k];
+        other[k] = make_float2(__shfl_xor_sync(0xffffffffu, gives.x, 1), __shfl_xor_sync(0xffffffffu, gives.y, 1));
+      }
+      const float4 mine = make_float4(own[0].x, own[0].y, own[1].x, own[1].y),
+                   its = make_float4(other[0].x, other[0].y, other[1].x, other[1].y);
+      float4* to4 = reinterpret_cast<float4*>(p + e0 - (odd ? 4 : 0));         // even: 0 and 8, odd: 4 and 12 from the pair's first
+      to4[0] = odd ? its : mine;
+      to4[2] = odd ? mine : its;
     } else {
       const uint32_t rw[4] = {random.x, random.y, random.z, random.w};
       uint32_t w[4];
