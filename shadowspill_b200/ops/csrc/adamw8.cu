@@ -11,11 +11,12 @@
 // The new moments are formed in fp32, one rounding to an operation (no contraction), so that the codes rounded to nearest
 // are those of the same operations anywhere else; the parameter's step uses them before they are rounded.
 //
-// Bound by memory: 10 bytes and 1/64 an element in bf16, 218 M elements in 330 us, 6.6 TB/s, with the moments and parameters rounded to nearest; with
+// Bound by memory: 10 bytes and 1/64 an element in bf16, 218 M elements in 330 us, 6.6 TB/s, with the moments and parameters rounded to nearest (fp32: 16 bytes, 527 us); with
 // random bits 418 us, three Philox calls to eight elements, where bf16 moments take 555.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
+#include <limits.h>
 #include <math.h>
 #include <stdint.h>
 
@@ -348,7 +349,7 @@ adamw8_kernel(const __grid_constant__ Table8 tab, Args8 a) {
       r_exp = x.r_exp;
     }
   }
-  for (; i < mine; ++i) {                        // a tensor's last block, or one off the boundaries of the pieces
+  for (; i < mine; ++i) {                        // a tensor's last block, or one off the boundaries of the pieces (50 M elements: 303 us, on them 87)
     const long long e0 = (first + static_cast<long long>(i) * A8_WARPS) * A8_BLOCK + lane * 8;
     x.m = x.r = make_uint2(0, 0);
     x.m_exp = __shfl_sync(0xffffffffu, m_exp, i);
@@ -423,9 +424,18 @@ int ss_adamw8_many(const long long* tensors, int count, int p_f32, int g_f32, co
   a.grad_scale = (float)grad_scale;
   a.one = 1.f;
   a.seed = static_cast<unsigned long long>(seed) ^ (0x9E3779B97F4A7C15ull * (unsigned long long)(step + 1));
-  // one wave of the three CTAs that fit on an SM, until their runs are long enough to hide their start
-  long long run = (total + 148 * 24 - 1) / (148 * 24);
-  run = run < 1 ? 1 : run > 16 ? 16 : run;
+  // One wave of the three CTAs that fit on an SM while no warp walks more than 16 blocks; then the run from 8
+  // on that leaves the last wave fullest (20 M elements: runs of 16 are 1.4 waves, 43 us in bf16 and 67 in fp32, of 11 two waves, 39.5 and 57; from 218 M
+  // on it makes no difference).
+  const long long each = (total + 148 * 24 - 1) / (148 * 24);
+  long long run = each < 1 ? 1 : each;
+  if (each > 16) {
+    long long least = LLONG_MAX;
+    for (long long r = 8; r <= 16; ++r) {
+      const long long walked = (each + r - 1) / r * r;
+      if (walked <= least) { least = walked; run = r; }
+    }
+  }
   for (int done = 0; done < count;) {
     Table8 tab;
     tab.count = 0;
