@@ -225,17 +225,26 @@ __device__ void finish_pair(int p, const Rows& rows, const PairArgs& a, const Wo
   const int from = rows.bound(2 * p), between = rows.bound(2 * p + 1), end = rows.bound(2 * p + 2);
   double sum[2] = {0.0, 0.0}, mass[2] = {0.0, 0.0};
   bool any0 = false, any1 = false;
-#pragma unroll 8
-  for (int r = from + rank; r < end; r += TEAM) {
-    const double ratio = __ldcg(work.ratio + r);
-    const float w = __ldcg(work.weight + r);
-    const int side = r >= between;
-    sum[0] += side ? 0.0 : ratio;
-    sum[1] += side ? ratio : 0.0;
-    mass[0] += side ? 0.f : w;
-    mass[1] += side ? w : 0.f;
-    any0 = any0 || (!side && w != 0.f);
-    any1 = any1 || (side && w != 0.f);
+  constexpr int AT_ONCE = 8;                     // loads on their way, the last few of them too
+  for (int r0 = from + rank; r0 < end; r0 += AT_ONCE * TEAM) {
+    double ratio[AT_ONCE];
+    float w[AT_ONCE];
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const int r = r0 + i * TEAM;
+      ratio[i] = r < end ? __ldcg(work.ratio + r) : 0.0;
+      w[i] = r < end ? __ldcg(work.weight + r) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const int side = r0 + i * TEAM >= between;
+      sum[0] += side ? 0.0 : ratio[i];
+      sum[1] += side ? ratio[i] : 0.0;
+      mass[0] += side ? 0.f : w[i];
+      mass[1] += side ? w[i] : 0.f;
+      any0 = any0 || (!side && w[i] != 0.f);
+      any1 = any1 || (side && w[i] != 0.f);
+    }
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -320,7 +329,7 @@ __global__ void clear_counters_kernel(int* words, int n) {
 // the cycles and half the issue slots; without exponentials it would be 122. Loads through a ring in shared memory, a part
 // of the exponentials by multiply-adds and blocks that stay while one warp finishes rows for the others were no faster.
 template <class L, int TEAM>
-__global__ void __launch_bounds__(Team<TEAM>::BLOCK)
+__global__ void __launch_bounds__(Team<TEAM>::BLOCK, TEAM == 512 ? 3 : 1)      // 512: 2 otherwise
 preference_rows_kernel(const L* logits, long long ld, bool aligned, Rows rows, PairArgs a, Work work, float* logp, float* sums,
                        float* loss_sum) {
   constexpr int WARPS = TEAM / 32;
@@ -525,20 +534,17 @@ int preference(const L* logits, long long ld, const Rows& rows, const PairArgs& 
     launch_chained(preference_grad_kernel<L, decltype(team)::value>, (rows.R + T::ROWS - 1) / T::ROWS, T::BLOCK, 0, s, logits, ld,
                    rows.targets, work, rows.R, rows.V, grad, ldg);
   };
-  // A row's team grows until the block has threads enough for the GPU and no thread has less than four pieces. Whole calls, us, by team of 32 /
-  // 128 / 256 / 512 / 1024, without the gradient: 8,000 rows of 2,500 words 40 / 45 / 63 / 128 / 340; 1,000 of 5,000 35 / 16 / 18 / 27 / 51;
-  // 4,096 of 128,256 - / 148 / 150 / 184 / 295; 200 of 151,936 - / 47 / 35 / 29 / 29.
+  // A row's team grows while all rows have a place on the GPU in teams of the next size and no thread has less than four pieces then. Calls without
+  // the gradient, us, by team of 32 / 128 / 256 / 512: 8,000 rows of 2,500 words 40 / 48 / 73 / 128; 2,000 of 4,096 19.6 / 21.5 / 28;
+  // 600 of 8,192 21.5 / 17.4 / 17.4; 1,021 of 50,304 63 / 37 / 43 / 49; 4,096 of 128,256 - / 148 / 150 / 184; 250 of 128,256 - / 45 / 35 / 31 (1,024: 41).
+  const int places[3][2] = {{128, 148 * 8}, {256, 148 * 5}, {512, 148 * 3}};
   int team = pieces <= 1024 ? 32 : 128;
-  while (team < 1024 && static_cast<long long>(rows.R) * team < 148 * 1024) {
-    const int next = team == 32 ? 128 : 2 * team;
-    if (pieces < 4 * next) break;
-    team = next;
-  }
+  for (const auto& [next, rows_at_once] : places)
+    if (next > team && rows.R <= rows_at_once && pieces >= 4 * next) team = next;
   if (team == 32) statistics(std::integral_constant<int, 32>());
   else if (team == 128) statistics(std::integral_constant<int, 128>());
   else if (team == 256) statistics(std::integral_constant<int, 256>());
-  else if (team == 512) statistics(std::integral_constant<int, 512>());
-  else statistics(std::integral_constant<int, 1024>());
+  else statistics(std::integral_constant<int, 512>());
   if (grad == nullptr || rows.R == 0) return (int)cudaGetLastError();
   // The gradient has nothing to reduce: by length alone. 8,000 rows of 1,000 words 39 / 41 / 45 / 60 / 93; 8,192 of 5,000 72 / 69 / 78 / 100 / 135;
   // 2,000 of 20,000 69 / 60 / 60 / 64 / 80; 4,096 of 128,256 466 / 454 / 442 / 429 / 457.
