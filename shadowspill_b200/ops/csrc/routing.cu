@@ -216,8 +216,8 @@ __device__ __forceinline__ void load_row(const L* row, int first, int E, bool ve
   for (int i = 0; i < PER; ++i) v[i] = first + i < E ? load_logit(row + first + i) : -INFINITY;
 }
 
-// LANES to a token, PER consecutive experts to a lane. Bound by instructions: 8,192 tokens of 64 experts take 10.4 us (2 of them for
-// clearing the counts), of 256 with a bias 22.0, and 65,537 of 512 in groups 129 us, 1,300 instructions a token with 60 % of the issue slots
+// LANES to a token, PER consecutive experts to a lane. Bound by instructions: 8,192 tokens of 64 experts take 9 us, of 256
+// with a bias 19, and 65,537 of 512 in groups 128 us, 1,300 instructions a token with 60 % of the issue slots
 // used; their memory would take 0.5, 1.4 and 11.
 //
 // The k-th largest of the lanes' own maxima bounds the k-th largest key from below: the keys from it on, a dozen where k
@@ -528,8 +528,8 @@ select_experts_kernel(const L* logits, bool vectors, bool bias_vectors, RouteArg
       atomicAdd(&hist[mine], 1);
     }
   }
-  chain_release();
   if (!alone) chain_wait();
+  chain_release();
   __syncthreads();
   for (int e = threadIdx.x; e < a.E; e += RT_THREADS) {
     if (alone) counts[e] = hist[e];
