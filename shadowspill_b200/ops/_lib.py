@@ -163,7 +163,8 @@ def check_status(device: torch.device | int | None = None) -> None:
 
 
 # kernels launched by one successful call of each launcher (attention backward:
-# delta + dQ + dKV; sum of squares: partials + final; preference loss: rows + gradient)
+# delta + dQ + dKV; sum of squares: partials + final; preference loss: rows + gradient). What only clears a call's
+# counters is not counted.
 _KERNELS_PER_CALL = {"ss_attn_bwd": 3, "ss_attn_bwd_g": 3, "ss_sumsq": 2, "ss_preference with its gradient": 2}
 _by_entry: dict[str, int] = {}
 

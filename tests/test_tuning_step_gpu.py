@@ -138,3 +138,43 @@ def test_a_step_of_all_three_against_autograd():
 
 def router_before(before):
     return before[0].detach().float()
+
+
+def test_calls_one_behind_the_other_see_what_came_before():
+    """Kernels of these operators start beside the one before them: inputs written and buffers reused just ahead of every call."""
+    g = torch.Generator(device=DEV).manual_seed(30)
+    logits = [torch.randn(3000, 64, generator=g, device=DEV) for _ in range(30)]
+    words = [torch.randn(700, 4000, generator=g, device=DEV).bfloat16() for _ in range(30)]
+    t = torch.randint(0, 4000, (700,), generator=g, device=DEV)
+    cu = torch.arange(0, 701, 35, dtype=torch.int32, device=DEV)
+    x, y = torch.empty_like(logits[0]), torch.empty_like(words[0])
+    results = []
+    for wait in (True, False):
+        p = torch.ones(300_001, device=DEV, dtype=torch.bfloat16)
+        state = F.moments8(p.numel(), DEV)
+        kept = []
+        torch.cuda.synchronize()
+        for i in range(30):
+            steps = []
+
+            def done(*tensors):
+                steps.extend(v.clone() for v in tensors)
+                if wait:
+                    torch.cuda.synchronize()
+            x.copy_(logits[i])
+            ids, w, counts = routing.select_experts(x, 6, scoring="sigmoid")
+            done(ids, w, counts)
+            done(routing.select_experts_bwd(x, ids, w, scoring="sigmoid"))
+            del ids, w, counts
+            y.copy_(words[i])
+            loss = torch.zeros(1, device=DEV)
+            F.preference_(y, t, None, cu, loss)
+            done(y, loss)
+            F.adamw8_many_([(p, y.view(-1)[:300_001], *state, 0)], lr=1e-2, step=i + 1)
+            done(p, *(v.view(torch.uint8) for v in state))
+            x.zero_()
+            y.zero_()
+            kept.append(steps)
+        torch.cuda.synchronize()
+        results.append(kept)
+    assert all(torch.equal(a, b) for one, other in zip(*results) for a, b in zip(one, other))
