@@ -20,6 +20,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "chained_launch.cuh"
 #include "launchers.h"
 
@@ -36,7 +38,6 @@ struct Tensor8 {
   long long n;
   unsigned long long offset;   // global element offset of the range: what the random bits are drawn by
   int first;                   // the launch's first CTA of this tensor
-  int vectors;                 // are all pointers on the boundaries of their 8-element pieces?
 };
 struct Table8 {
   Tensor8 t[A8_TENSORS];
@@ -251,7 +252,10 @@ template <class P, class G> struct Ring8 {
   static constexpr int P16 = sizeof(P) / 2, G16 = sizeof(G) / 2;       // 16-byte pieces of a lane
   static constexpr int STAGE = 32 * (16 * P16 + 16 * G16 + 16), STAGES = 48 * 1024 / A8_WARPS / STAGE;
 };
-template <class P, class G, bool SR_PARAM, bool SR_STATE>
+// STAGED: tensors off the boundaries of their pieces. Neighbouring elements go by neighbouring lanes, and through shared memory to the eight
+// of a lane and back: 50 M bf16 elements, one element off, 156 us (by each lane's elements 303, on the boundaries 85). A kernel of its own: with
+// this in the other one a layer of 218 M elements took 376 us instead of 361.
+template <class P, class G, bool SR_PARAM, bool SR_STATE, bool STAGED>
 __global__ void __launch_bounds__(A8_THREADS, 3)
 adamw8_kernel(const __grid_constant__ Table8 tab, Args8 a) {
   using Ring = Ring8<P, G>;
@@ -268,7 +272,7 @@ adamw8_kernel(const __grid_constant__ Table8 tab, Args8 a) {
   P* const p = static_cast<P*>(t.p);
   const G* const g = static_cast<const G*>(t.g);
   const long long first = static_cast<long long>(blockIdx.x - t.first) * tab.run * A8_WARPS + warp;
-  const long long blocks = (t.n + A8_BLOCK - 1) / A8_BLOCK, whole = t.vectors ? t.n / A8_BLOCK : 0;
+  const long long blocks = (t.n + A8_BLOCK - 1) / A8_BLOCK, whole = STAGED ? 0 : t.n / A8_BLOCK;
   auto walked = [&](long long end) {             // blocks of this warp's run before `end`
     const long long n = first < end ? (end - first + A8_WARPS - 1) / A8_WARPS : 0;
     return n < tab.run ? static_cast<int>(n) : tab.run;
@@ -296,88 +300,152 @@ adamw8_kernel(const __grid_constant__ Table8 tab, Args8 a) {
   Eight out;
   uint4 random;
   Read8<P, G> x = {};
-  for (int i = 0; i < Ring::STAGES - 1; ++i) fetch(i);
-  int i = 0;
-  for (; i < full; ++i) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(Ring::STAGES - 2) : "memory");
-    const long long e0 = (first + static_cast<long long>(i) * A8_WARPS) * A8_BLOCK + lane * 8;
-    __syncwarp();                                // copies of other lanes, where a lane's eight elements are two pieces
-    const uint4* q = reinterpret_cast<const uint4*>(ring[warp][i % Ring::STAGES]);
-    x.p.load(q + lane * Ring::P16);
-    q += 32 * Ring::P16;
-    x.g.load(q + lane * Ring::G16);
-    const uint2* c = reinterpret_cast<const uint2*>(q + 32 * Ring::G16) + lane;
-    x.m = c[0];
-    x.r = c[32];
-    x.m_exp = __shfl_sync(0xffffffffu, m_exp, i);
-    x.r_exp = __shfl_sync(0xffffffffu, r_exp, i);
-    fetch(i + Ring::STAGES - 1);                 // into the stage of the block before this one
-    update8<SR_PARAM, SR_STATE>(x, a, t.offset + static_cast<unsigned long long>(e0), out, random);
-    if (sizeof(P) == 4) {
-      // two lanes write the halves of the even one's eight elements, then those of the odd one's: whole sectors
-      const bool odd = lane & 1;
-      float2 own[2], other[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const float2 gives = odd ? out.v[k] : out.v[2 + k];
-        own[k] = odd ? out.v[2 + k] : out.v[k];
-        other[k] = make_float2(__shfl_xor_sync(0xffffffffu, gives.x, 1), __shfl_xor_sync(0xffffffffu, gives.y, 1));
-      }
-      const float4 mine = make_float4(own[0].x, own[0].y, own[1].x, own[1].y),
-                   its = make_float4(other[0].x, other[0].y, other[1].x, other[1].y);
-      float4* to4 = reinterpret_cast<float4*>(p + e0 - (odd ? 4 : 0));         // even: 0 and 8, odd: 4 and 12 from the pair's first
-      to4[0] = odd ? its : mine;
-      to4[2] = odd ? mine : its;
-    } else {
-      const uint32_t rw[4] = {random.x, random.y, random.z, random.w};
-      uint32_t w[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (SR_PARAM) {
-          w[k] = bf16_bits<true>(out.v[k].x, rw[k] & 0xffffu) | bf16_bits<true>(out.v[k].y, rw[k] >> 16) << 16;
-        } else {
-          const __nv_bfloat162 two = __float22bfloat162_rn(out.v[k]);
-          w[k] = *reinterpret_cast<const uint32_t*>(&two);
-        }
-      }
-      *reinterpret_cast<uint4*>(p + e0) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    *reinterpret_cast<uint2*>(t.m + e0) = x.m;
-    *reinterpret_cast<uint2*>(t.r + e0) = x.r;
-    if (lane == i) {
-      m_exp = x.m_exp;
-      r_exp = x.r_exp;
-    }
-  }
-  for (; i < mine; ++i) {                        // a tensor's last block, or one off the boundaries of the pieces (50 M elements: 303 us, on them 87)
-    const long long e0 = (first + static_cast<long long>(i) * A8_WARPS) * A8_BLOCK + lane * 8;
-    x.m = x.r = make_uint2(0, 0);
-    x.m_exp = __shfl_sync(0xffffffffu, m_exp, i);
-    x.r_exp = __shfl_sync(0xffffffffu, r_exp, i);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const bool in = e0 + e < t.n;
-      x.p.set(e, in ? p[e0 + e] : P(0.f));
-      x.g.set(e, in ? g[e0 + e] : G(0.f));
-      const uint32_t m = in ? t.m[e0 + e] : 0, r = in ? t.r[e0 + e] : 0;
-      (e < 4 ? x.m.x : x.m.y) |= m << (8 * (e & 3));
-      (e < 4 ? x.r.x : x.r.y) |= r << (8 * (e & 3));
-    }
-    update8<SR_PARAM, SR_STATE>(x, a, t.offset + static_cast<unsigned long long>(e0), out, random);
+  auto rounded = [&] {                           // the new parameters in bf16
     const uint32_t rw[4] = {random.x, random.y, random.z, random.w};
+    uint32_t w[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (e0 + e >= t.n) continue;
-      const float f = (e & 1) ? out.v[e >> 1].y : out.v[e >> 1].x;
-      if (sizeof(P) == 4) reinterpret_cast<float*>(p)[e0 + e] = f;
-      else reinterpret_cast<unsigned short*>(p)[e0 + e] =
-          static_cast<unsigned short>(bf16_bits<SR_PARAM>(f, (e & 1) ? rw[e >> 1] >> 16 : rw[e >> 1] & 0xffffu));
-      t.m[e0 + e] = static_cast<uint8_t>((e < 4 ? x.m.x : x.m.y) >> (8 * (e & 3)));
-      t.r[e0 + e] = static_cast<uint8_t>((e < 4 ? x.r.x : x.r.y) >> (8 * (e & 3)));
+    for (int k = 0; k < 4; ++k) {
+      if (SR_PARAM) {
+        w[k] = bf16_bits<true>(out.v[k].x, rw[k] & 0xffffu) | bf16_bits<true>(out.v[k].y, rw[k] >> 16) << 16;
+      } else {
+        const __nv_bfloat162 two = __float22bfloat162_rn(out.v[k]);
+        w[k] = *reinterpret_cast<const uint32_t*>(&two);
+      }
     }
-    if (lane == i) {
-      m_exp = x.m_exp;
-      r_exp = x.r_exp;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  if constexpr (STAGED) {
+    int i = 0;
+    P* const sp = reinterpret_cast<P*>(ring[warp][0]);
+    G* const sg = reinterpret_cast<G*>(sp + A8_BLOCK);
+    uint8_t *const sm = reinterpret_cast<uint8_t*>(sg + A8_BLOCK), *const sr = sm + A8_BLOCK;
+    for (; i < mine; ++i) {
+      const long long block = (first + static_cast<long long>(i) * A8_WARPS) * A8_BLOCK;
+      const int n = static_cast<int>(min(t.n - block, static_cast<long long>(A8_BLOCK)));
+      P pe[8];
+      G ge[8];
+      uint8_t me[8], re[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int e = lane + 32 * k;
+        pe[k] = e < n ? p[block + e] : P(0.f);
+        ge[k] = e < n ? g[block + e] : G(0.f);
+        me[k] = e < n ? t.m[block + e] : uint8_t(0);
+        re[k] = e < n ? t.r[block + e] : uint8_t(0);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int e = lane + 32 * k;
+        sp[e] = pe[k];
+        sg[e] = ge[k];
+        sm[e] = me[k];
+        sr[e] = re[k];
+      }
+      __syncwarp();
+      x.p.load(reinterpret_cast<const uint4*>(sp) + lane * Ring::P16);
+      x.g.load(reinterpret_cast<const uint4*>(sg) + lane * Ring::G16);
+      x.m = reinterpret_cast<const uint2*>(sm)[lane];
+      x.r = reinterpret_cast<const uint2*>(sr)[lane];
+      x.m_exp = __shfl_sync(0xffffffffu, m_exp, i);
+      x.r_exp = __shfl_sync(0xffffffffu, r_exp, i);
+      update8<SR_PARAM, SR_STATE>(x, a, t.offset + static_cast<unsigned long long>(block + lane * 8), out, random);
+      if (sizeof(P) == 4) {
+        float4* to4 = reinterpret_cast<float4*>(sp) + 2 * lane;
+        to4[0] = make_float4(out.v[0].x, out.v[0].y, out.v[1].x, out.v[1].y);
+        to4[1] = make_float4(out.v[2].x, out.v[2].y, out.v[3].x, out.v[3].y);
+      } else {
+        reinterpret_cast<uint4*>(sp)[lane] = rounded();
+      }
+      reinterpret_cast<uint2*>(sm)[lane] = x.m;
+      reinterpret_cast<uint2*>(sr)[lane] = x.r;
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int e = lane + 32 * k;
+        if (e >= n) continue;
+        p[block + e] = sp[e];
+        t.m[block + e] = sm[e];
+        t.r[block + e] = sr[e];
+      }
+      __syncwarp();
+      if (lane == i) {
+        m_exp = x.m_exp;
+        r_exp = x.r_exp;
+      }
+    }
+  } else {
+    for (int i = 0; i < Ring::STAGES - 1; ++i) fetch(i);
+    int i = 0;
+    for (; i < full; ++i) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(Ring::STAGES - 2) : "memory");
+      const long long e0 = (first + static_cast<long long>(i) * A8_WARPS) * A8_BLOCK + lane * 8;
+      __syncwarp();                                // copies of other lanes, where a lane's eight elements are two pieces
+      const uint4* q = reinterpret_cast<const uint4*>(ring[warp][i % Ring::STAGES]);
+      x.p.load(q + lane * Ring::P16);
+      q += 32 * Ring::P16;
+      x.g.load(q + lane * Ring::G16);
+      const uint2* c = reinterpret_cast<const uint2*>(q + 32 * Ring::G16) + lane;
+      x.m = c[0];
+      x.r = c[32];
+      x.m_exp = __shfl_sync(0xffffffffu, m_exp, i);
+      x.r_exp = __shfl_sync(0xffffffffu, r_exp, i);
+      fetch(i + Ring::STAGES - 1);                 // into the stage of the block before this one
+      update8<SR_PARAM, SR_STATE>(x, a, t.offset + static_cast<unsigned long long>(e0), out, random);
+      if (sizeof(P) == 4) {
+        // two lanes write the halves of the even one's eight elements, then those of the odd one's: whole sectors
+        const bool odd = lane & 1;
+        float2 own[2], other[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float2 gives = odd ? out.v[k] : out.v[2 + k];
+          own[k] = odd ? out.v[2 + k] : out.v[k];
+          other[k] = make_float2(__shfl_xor_sync(0xffffffffu, gives.x, 1), __shfl_xor_sync(0xffffffffu, gives.y, 1));
+        }
+        const float4 mine = make_float4(own[0].x, own[0].y, own[1].x, own[1].y),
+                     its = make_float4(other[0].x, other[0].y, other[1].x, other[1].y);
+        float4* to4 = reinterpret_cast<float4*>(p + e0 - (odd ? 4 : 0));         // even: 0 and 8, odd: 4 and 12 from the pair's first
+        to4[0] = odd ? its : mine;
+        to4[2] = odd ? mine : its;
+      } else {
+        *reinterpret_cast<uint4*>(p + e0) = rounded();
+      }
+      *reinterpret_cast<uint2*>(t.m + e0) = x.m;
+      *reinterpret_cast<uint2*>(t.r + e0) = x.r;
+      if (lane == i) {
+        m_exp = x.m_exp;
+        r_exp = x.r_exp;
+      }
+    }
+    for (; i < mine; ++i) {                        // a tensor's last block
+      const long long e0 = (first + static_cast<long long>(i) * A8_WARPS) * A8_BLOCK + lane * 8;
+      x.m = x.r = make_uint2(0, 0);
+      x.m_exp = __shfl_sync(0xffffffffu, m_exp, i);
+      x.r_exp = __shfl_sync(0xffffffffu, r_exp, i);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool in = e0 + e < t.n;
+        x.p.set(e, in ? p[e0 + e] : P(0.f));
+        x.g.set(e, in ? g[e0 + e] : G(0.f));
+        const uint32_t m = in ? t.m[e0 + e] : 0, r = in ? t.r[e0 + e] : 0;
+        (e < 4 ? x.m.x : x.m.y) |= m << (8 * (e & 3));
+        (e < 4 ? x.r.x : x.r.y) |= r << (8 * (e & 3));
+      }
+      update8<SR_PARAM, SR_STATE>(x, a, t.offset + static_cast<unsigned long long>(e0), out, random);
+      const uint32_t rw[4] = {random.x, random.y, random.z, random.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (e0 + e >= t.n) continue;
+        const float f = (e & 1) ? out.v[e >> 1].y : out.v[e >> 1].x;
+        if (sizeof(P) == 4) reinterpret_cast<float*>(p)[e0 + e] = f;
+        else reinterpret_cast<unsigned short*>(p)[e0 + e] =
+            static_cast<unsigned short>(bf16_bits<SR_PARAM>(f, (e & 1) ? rw[e >> 1] >> 16 : rw[e >> 1] & 0xffffu));
+        t.m[e0 + e] = static_cast<uint8_t>((e < 4 ? x.m.x : x.m.y) >> (8 * (e & 3)));
+        t.r[e0 + e] = static_cast<uint8_t>((e < 4 ? x.r.x : x.r.y) >> (8 * (e & 3)));
+      }
+      if (lane == i) {
+        m_exp = x.m_exp;
+        r_exp = x.r_exp;
+      }
     }
   }
   if (lane < mine) {
@@ -386,15 +454,15 @@ adamw8_kernel(const __grid_constant__ Table8 tab, Args8 a) {
   }
 }
 
-template <class P, class G>
-int launch8(const Table8& tab, const Args8& a, int runs, int sr_param, int sr_state, cudaStream_t s) {
+template <class P, class G, bool STAGED>
+int launch8(const Table8& tab, const Args8& a, int ctas, int sr_param, int sr_state, cudaStream_t s) {
   auto go = [&](auto kern) {
-    launch_chained(kern, runs, A8_THREADS, 0, s, tab, a);
+    launch_chained(kern, ctas, A8_THREADS, 0, s, tab, a);
     return (int)cudaGetLastError();
   };
   if (sizeof(P) == 2 && sr_param)
-    return sr_state ? go(adamw8_kernel<P, G, true, true>) : go(adamw8_kernel<P, G, true, false>);
-  return sr_state ? go(adamw8_kernel<P, G, false, true>) : go(adamw8_kernel<P, G, false, false>);
+    return sr_state ? go(adamw8_kernel<P, G, true, true, STAGED>) : go(adamw8_kernel<P, G, true, false, STAGED>);
+  return sr_state ? go(adamw8_kernel<P, G, false, true, STAGED>) : go(adamw8_kernel<P, G, false, false, STAGED>);
 }
 
 }  // namespace
@@ -436,32 +504,39 @@ int ss_adamw8_many(const long long* tensors, int count, int p_f32, int g_f32, co
       if (walked <= least) { least = walked; run = r; }
     }
   }
-  for (int done = 0; done < count;) {
-    Table8 tab;
-    tab.count = 0;
-    tab.run = (int)run;
-    long long runs = 0;
-    for (; done < count && tab.count < A8_TENSORS; ++done) {
-      const long long* t = tensors + 8 * done;
-      if (t[6] == 0) continue;
-      const long long mine = ((t[6] + A8_BLOCK - 1) / A8_BLOCK + run * A8_WARPS - 1) / (run * A8_WARPS);
-      if (runs + mine > 0x3fffffff) {
-        if (tab.count == 0) return -2;
-        break;
+  // are all pointers of a tensor on the boundaries of their 8-element pieces?
+  auto whole = [&](const long long* t) { return t[0] % 16 == 0 && t[1] % 16 == 0 && t[2] % 8 == 0 && t[3] % 8 == 0; };
+  auto launches = [&](auto staged) {
+    for (int done = 0; done < count;) {
+      Table8 tab;
+      tab.count = 0;
+      tab.run = (int)run;
+      long long ctas = 0;
+      for (; done < count && tab.count < A8_TENSORS; ++done) {
+        const long long* t = tensors + 8 * done;
+        if (t[6] == 0 || whole(t) == decltype(staged)::value) continue;
+        const long long mine = ((t[6] + A8_BLOCK - 1) / A8_BLOCK + run * A8_WARPS - 1) / (run * A8_WARPS);
+        if (ctas + mine > 0x3fffffff) {
+          if (tab.count == 0) return -2;
+          break;
+        }
+        tab.t[tab.count++] = {(void*)t[0], (const void*)t[1], (uint8_t*)t[2], (uint8_t*)t[3], (uint8_t*)t[4], (uint8_t*)t[5],
+                              t[6], (unsigned long long)t[7], (int)ctas};
+        ctas += mine;
       }
-      const int vectors = t[0] % 16 == 0 && t[1] % 16 == 0 && t[2] % 8 == 0 && t[3] % 8 == 0;
-      tab.t[tab.count++] = {(void*)t[0], (const void*)t[1], (uint8_t*)t[2], (uint8_t*)t[3], (uint8_t*)t[4], (uint8_t*)t[5],
-                            t[6], (unsigned long long)t[7], (int)runs, vectors};
-      runs += mine;
+      if (tab.count == 0) break;
+      constexpr bool STAGED = decltype(staged)::value;
+      cudaStream_t s = (cudaStream_t)stream;
+      const int n = (int)ctas;
+      const int e = p_f32 ? (g_f32 ? launch8<float, float, STAGED>(tab, a, n, sr_param, sr_state, s)
+                                   : launch8<float, bf16, STAGED>(tab, a, n, sr_param, sr_state, s))
+                          : (g_f32 ? launch8<bf16, float, STAGED>(tab, a, n, sr_param, sr_state, s)
+                                   : launch8<bf16, bf16, STAGED>(tab, a, n, sr_param, sr_state, s));
+      if (e) return e;
     }
-    if (tab.count == 0) break;
-    cudaStream_t s = (cudaStream_t)stream;
-    const int e = p_f32 ? (g_f32 ? launch8<float, float>(tab, a, (int)runs, sr_param, sr_state, s)
-                                 : launch8<float, bf16>(tab, a, (int)runs, sr_param, sr_state, s))
-                        : (g_f32 ? launch8<bf16, float>(tab, a, (int)runs, sr_param, sr_state, s)
-                                 : launch8<bf16, bf16>(tab, a, (int)runs, sr_param, sr_state, s));
-    if (e) return e;
-  }
-  return 0;
+    return 0;
+  };
+  const int e = launches(std::false_type());
+  return e ? e : launches(std::true_type());
 }
 }  // extern "C"
