@@ -562,13 +562,49 @@ __global__ void clear_counts_kernel(int* counts, int E) {
   for (int e = threadIdx.x; e < E; e += blockDim.x) counts[e] = 0;
 }
 
-// With c_j the picked scores, S their sum: dc_j = scale / S (dw_j - sum_i dw_i c_i / S) or scale dw_j, and
-//   sigmoid  dx_e = dc_e s_e (1 - s_e);   softmax  dx_e = s_e (dc_e - sum_j dc_j s_j), whose sum is zero if renormalised.
-// A warp to a token: the chain of picks, scores and sums while other warps store zeros. 65,537 x 512 bf16 in 18.8 us (67 MB, 3.6 TB/s);
-// 8,192 x 64 in 4.4, of which a launch is half.
-template <class L>
-__global__ void __launch_bounds__(RT_THREADS)
+// A row by its lanes: pieces of N elements, lane + 32 c the c-th of a lane, so that an instruction takes consecutive ones. WHOLE: the row starts on a
+// piece's boundary and has whole pieces; by element otherwise.
+template <int PER, bool WHOLE, class L> struct Spread {
+  static constexpr int MOST = 16 / static_cast<int>(sizeof(L)), N = !WHOLE ? 1 : PER < MOST ? PER : MOST;
+  using Piece = std::conditional_t<N * sizeof(L) == 16, uint4, std::conditional_t<N * sizeof(L) == 8, uint2, std::conditional_t<N * sizeof(L) == 4, uint32_t, uint16_t>>>;
+  __device__ static int first(int lane, int c) { return (lane + 32 * c) * N; }
+  __device__ static void load(const L* row, int lane, int E, float (&v)[PER]) {
+#pragma unroll
+    for (int c = 0; c < PER / N; ++c) {
+      const int e = first(lane, c);
+      alignas(16) L piece[N];
+      if (e < E) *reinterpret_cast<Piece*>(piece) = *reinterpret_cast<const Piece*>(row + e);
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[c * N + i] = e < E ? load_logit(piece + i) : -INFINITY;
+    }
+  }
+  __device__ static void store(L* row, int lane, int E, const float (&v)[PER]) {
+#pragma unroll
+    for (int c = 0; c < PER / N; ++c) {
+      const int e = first(lane, c);
+      alignas(16) L piece[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) store_logit(piece + i, v[c * N + i]);
+      if (e < E) *reinterpret_cast<Piece*>(row + e) = *reinterpret_cast<const Piece*>(piece);
+    }
+  }
+};
+
+// With c_j the picked scores, S = sum_j c_j + 1e-20, A = sum_j dw_j c_j / S: dc_j = scale (dw_j - A) / S, or scale dw_j as they are, and
+//   sigmoid  dx_e = dc_e s_e (1 - s_e);   softmax  dx_e = s_e (dc_e - B) with B = sum_j dc_j s_j, which is scale A 1e-20 / S if renormalised.
+// B counts there where the picks' scores are next to nothing: a bias can bring that about, and the row's largest logit shows it. With a pick
+// within 20 of that, the picks hold e^-20 / 512 = 4e-12 of the row or more, 1e-20 is under the rounding of their sum, and scores are taken
+// relative to the largest pick; experts that were not picked get zero.
+// A warp to a token. 65,537 x 512 bf16: sigmoid 22 us (67 MB written), softmax renormalised 25.5 (67 MB read too, for the largest logit), not
+// renormalised 33 (an exponential for each, kept in registers). 8,192 x 256 fp32, sigmoid: 4.3, of which a launch is half.
+constexpr float PICKS_NEAR = 20.f;
+__device__ __forceinline__ float below(float x, float top) { return x == -INFINITY ? 0.f : exp_of(x - top); }
+enum { SIGMOID, SOFTMAX_RENORMALISED, SOFTMAX };
+constexpr int bwd_resident(int mode, int per) { return mode != SOFTMAX || per <= 4 ? 16 : per == 8 ? 12 : 10; }
+template <int MODE, int PER, bool WHOLE, class L>
+__global__ void __launch_bounds__(RT_THREADS, bwd_resident(MODE, PER))
 select_experts_bwd_kernel(const L* logits, RouteArgs a, const int* ids, const float* dweights, L* dlogits) {
+  using Row = Spread<PER, WHOLE, L>;
   chain_wait();
   chain_release();
   const int lane = threadIdx.x & 31;
@@ -577,43 +613,61 @@ select_experts_bwd_kernel(const L* logits, RouteArgs a, const int* ids, const fl
     L* out = dlogits + static_cast<long long>(t) * a.E;
     const bool pick = lane < a.k;
     const int id = pick ? ids[static_cast<long long>(t) * a.k + lane] : 0;
+    float v[PER], top = -INFINITY;
+    if (MODE != SIGMOID) {
+      Row::load(row, lane, a.E, v);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) top = fmaxf(top, v[i]);
+    }
     const bool in = pick && id >= 0 && id < a.E;
-    const float dw = in ? dweights[static_cast<long long>(t) * a.k + lane] : 0.f;
+    const float d = in ? a.scale * dweights[static_cast<long long>(t) * a.k + lane] : 0.f;
     const float x = in ? load_logit(row + id) : -INFINITY;
-    float top = 0.f, total = 1.f, s, inner = 0.f;
-    const bool whole = !a.sigmoid && !a.renormalize;
-    if (whole) {
-      top = -INFINITY;
-      for (int e = lane; e < a.E; e += 32) top = fmaxf(top, load_logit(row + e));
-      top = warp_max32(top);
-      float sum = 0.f;
-      for (int e = lane; e < a.E; e += 32) {
-        const float y = load_logit(row + e);
-        sum += y == -INFINITY ? 0.f : exp_of(y - top);
-      }
-      total = warp_sum32(sum);
-    } else if (!a.sigmoid) {
-      top = warp_max32(x);
-    }
-    float other = 0.f;
-    if (a.sigmoid) s = sigmoid_score(x, other);
-    else s = x == -INFINITY ? 0.f : quotient(expf(x - top), fmaxf(total, 1.f));
-    float d = a.scale * dw;
-    if (a.renormalize) {
-      const float sum = warp_sum32(s) + 1e-20f;
-      d = quotient(d - quotient(warp_sum32(d * s), sum), sum);
-    }
-    if (whole) {
-      inner = warp_sum32(d * s);
-      for (int e = lane; e < a.E; e += 32) {
-        const float y = load_logit(row + e);
-        store_logit(out + e, y == -INFINITY ? 0.f : -__fdividef(exp_of(y - top), fmaxf(total, 1.f)) * inner);
-      }
+    float total = 1.f, s, other = 0.f, inner = 0.f;
+    bool others = MODE == SOFTMAX;               // do experts that were not picked have gradients?
+    if (MODE == SIGMOID) {
+      s = sigmoid_score(x, other);
     } else {
-      for (int e = lane; e < a.E; e += 32) store_logit(out + e, 0.f);
+      float base = warp_max32(x);
+      top = warp_max32(top);
+      if (MODE == SOFTMAX_RENORMALISED) others = !(base >= top - PICKS_NEAR);
+      if (others) {
+        total = 0.f;
+        if (MODE == SOFTMAX) {
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            v[i] = below(v[i], top);
+            total += v[i];
+          }
+        } else {
+          for (int e = lane; e < a.E; e += 32) total += below(load_logit(row + e), top);
+        }
+        total = fmaxf(warp_sum32(total), 1.f);
+        base = top;
+      }
+      s = x == -INFINITY ? 0.f : quotient(expf(x - base), total);
+    }
+    float mine;                                  // dc_j s_j
+    if (a.renormalize) {
+      const float sum = warp_sum32(s) + 1e-20f, u = quotient(s, sum), mean = warp_sum32(d * u);
+      mine = (d - mean) * u;
+      if (others) inner = mean * quotient(1e-20f, sum);
+    } else {
+      mine = d * s;
+      if (MODE == SOFTMAX) inner = warp_sum32(mine);
+    }
+    const float each = others ? -quotient(inner, total) : 0.f;
+    if (MODE == SOFTMAX) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[i] *= each;
+      Row::store(out, lane, a.E, v);
+    } else if (others) {                         // hardly ever: read again instead of kept in registers
+      for (int e = lane; e < a.E; e += 32) store_logit(out + e, below(load_logit(row + e), top) * each);
+    } else {
+      const float zero[PER] = {};
+      Row::store(out, lane, a.E, zero);
     }
     __syncwarp();                                // the picks overwrite what another lane wrote above
-    if (in) store_logit(out + id, a.sigmoid ? d * s * other : s * (d - inner));
+    if (in) store_logit(out + id, MODE == SIGMOID ? mine * other : mine - s * inner);
   }
 }
 
@@ -674,13 +728,30 @@ int ss_select_experts_bwd(const void* logits, int bf16_logits, long long ld, con
   const RouteArgs a{T, E, k, 1, 1, sigmoid, renormalize, ld, scale, nullptr};
   if (!fits(a)) return -2;
   if (T == 0) return 0;
-  const int blocks = (T + RT_WARPS - 1) / RT_WARPS, grid = blocks < 148 * 16 ? blocks : 148 * 16;
-  auto go = [&](auto kern, auto* x) {
-    launch_chained(kern, grid, RT_THREADS, 0, (cudaStream_t)stream, x, a, ids, dweights, const_cast<std::remove_const_t<std::remove_pointer_t<decltype(x)>>*>(
-        reinterpret_cast<decltype(x)>(dlogits)));
+  const int per = (E + 31) / 32, blocks = (T + RT_WARPS - 1) / RT_WARPS;
+  auto go = [&](auto mode, auto n, auto whole, auto* x, auto* out) {
+    using X = std::remove_pointer_t<decltype(out)>;
+    const int most = 148 * bwd_resident(mode, n), grid = blocks < most ? blocks : most;
+    launch_chained(select_experts_bwd_kernel<decltype(mode)::value, decltype(n)::value, decltype(whole)::value, X>, grid, RT_THREADS, 0,
+                   (cudaStream_t)stream, x, a, ids, dweights, out);
+    return (int)cudaGetLastError();
   };
-  if (bf16_logits) go(select_experts_bwd_kernel<__nv_bfloat16>, (const __nv_bfloat16*)logits);
-  else go(select_experts_bwd_kernel<float>, (const float*)logits);
-  return (int)cudaGetLastError();
+  auto by_length = [&](auto mode, auto whole, auto* x, auto* out) {
+    if (per <= 2) return go(mode, std::integral_constant<int, 2>(), whole, x, out);
+    if (per <= 4) return go(mode, std::integral_constant<int, 4>(), whole, x, out);
+    if (per <= 8) return go(mode, std::integral_constant<int, 8>(), whole, x, out);
+    return go(mode, std::integral_constant<int, 16>(), whole, x, out);
+  };
+  auto by_mode = [&](auto whole, auto* x, auto* out) {
+    if (sigmoid) return by_length(std::integral_constant<int, SIGMOID>(), whole, x, out);
+    if (renormalize) return by_length(std::integral_constant<int, SOFTMAX_RENORMALISED>(), whole, x, out);
+    return by_length(std::integral_constant<int, SOFTMAX>(), whole, x, out);
+  };
+  auto by_type = [&](auto* x, auto* out) {
+    const bool whole = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld * sizeof(*x) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 &&
+                       E * sizeof(*x) % 16 == 0;
+    return whole ? by_mode(std::true_type(), x, out) : by_mode(std::false_type(), x, out);
+  };
+  return bf16_logits ? by_type((const __nv_bfloat16*)logits, (__nv_bfloat16*)dlogits) : by_type((const float*)logits, (float*)dlogits);
 }
 }  // extern "C"

@@ -47,3 +47,44 @@ def test_softmax_weights_far_below_the_top(renormalize):
         c = c / (c.sum(1, keepdim=True) + 1e-20)
         score, low = 2 * score, low * 1e20 * 5
     assert bool(((w - c).abs() <= score * c + low).all())
+
+
+@pytest.mark.parametrize("gap", [0.0, 10.0, 18.0, 21.0, 40.0, 46.0, 50.0, 60.0, 90.0])
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("E,k", [(16, 4), (64, 1), (65, 7), (512, 10)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradient_of_softmax_picks_far_below_the_top(gap, renormalize, E, k, dtype):
+    """A bias picks experts whose scores are nothing beside the row's largest, which is not picked: the sum that the weights
+    are divided by is then of the size of the 1e-20 beside it, and the others have gradients too."""
+    x, dw, scale = _rand(50, E, seed=E), _rand(50, k, seed=8), 2.5
+    x[:, 3] = x.amax(1) + gap
+    x = x.to(dtype)
+    bias = torch.zeros(E, device=DEV)
+    bias[4:4 + k] = 10.0
+    ids, w, _ = routing.select_experts(x, k, bias=bias, renormalize=renormalize, scale=scale)
+    assert torch.equal(ids.sort(1).values, torch.arange(4, 4 + k, device=DEV, dtype=torch.int32).expand(50, k))
+    got = routing.select_experts_bwd(x, ids, dw, renormalize=renormalize, scale=scale)
+    x64 = x.double().requires_grad_(True)
+    s = torch.softmax(x64, 1)
+    c = s.gather(1, ids.long())
+    want_w = scale * (c / (c.sum(1, keepdim=True) + 1e-20) if renormalize else c)
+    want = torch.autograd.grad(want_w, x64, dw.double())[0]
+    s, c, want_w = s.detach(), c.detach(), want_w.detach()
+    # A score: its argument, a difference of up to gap + 8, is rounded by half a step of that, the exponential by 2 steps, its
+    # row's sum by 16 together with the quotient. A weight has one above and one below the line; a gradient three such factors.
+    score = (gap + 8) / 2 * STEP + 18 * STEP
+    u = c / (c.sum(1, keepdim=True) + 1e-20) if renormalize else c
+    mean = (dw.double().abs() * u).sum(1, keepdim=True)
+    size = torch.zeros_like(s).scatter_(1, ids.long(), scale * u * (dw.double().abs() + (mean if renormalize else 0.0)))
+    inner = scale * mean * (1e-20 / (c.sum(1, keepdim=True) + 1e-20) if renormalize else 1.0)
+    size = size + s * inner
+    # scores under fp32's normal range keep steps of 2^-149, times 1e20 where that is all they are divided by; and 1e-20 of a sum
+    # that is 4e-12 or more (a pick within 20 of the top of 512) is below the rounding of the others and may be left out
+    low = 2.0 ** -149 * (1e20 if renormalize else 1.0) * scale
+    assert bool(((w - want_w).abs() <= 2 * score * want_w + 2 * k * low).all())
+    left = 2.5e-9 * scale * mean * s if renormalize else 0.0
+    # a gradient under the normal range is a multiple of the type's smallest step, half of which its rounding and that of a product that it
+    # is formed from are off by, however small dw is
+    least = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    allowed = 4 * score * size + left + torch.finfo(dtype).eps / 2 * want.abs() + 4 * k * low * dw.abs().sum(1, keepdim=True) + 2 * least
+    assert bool(((got.double() - want).abs() <= allowed).all())
