@@ -128,15 +128,17 @@ __device__ unsigned kept_groups(const F* keys, const RouteArgs& a, int lane, F& 
   return bits;
 }
 
-// A row's largest logit and its softmax's sum in 64 bits, of the lanes' own values where LANES share a row.
+// A row's softmax's sum in 64 bits, of the lanes' own values where LANES share a row: 1 for a row of -inf, NaN for one with a NaN or +inf, whose
+// keys are then all NaN.
+__device__ __forceinline__ double term64(float x, float top) { return x == -INFINITY ? 0.0 : exp(static_cast<double>(x) - top); }
 template <int LANES>
-__device__ __forceinline__ double sum64(float top, double part) {
+__device__ __forceinline__ double sum64(double part) {
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) part += __shfl_xor_sync(FULL, part, o);
-  return top > -INFINITY ? part : 1.0;
+  return part == 0.0 ? 1.0 : part;
 }
 __device__ __forceinline__ double key64(float x, float top, double total, const float* bias, int e, bool sigmoid) {
-  double v = sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(x))) : x == -INFINITY ? 0.0 : exp(static_cast<double>(x) - top) / total;
+  double v = sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(x))) : term64(x, top) / total;
   if (bias != nullptr) v += bias[e];
   return v == v ? v : -INFINITY;
 }
@@ -149,11 +151,8 @@ __device__ __noinline__ unsigned exact_keys(const L* row, const RouteArgs& a, do
   top = warp_max32(top);
   double part = 0.0;
   if (!a.sigmoid)
-    for (int e = lane; e < a.E; e += 32) {
-      const float x = load_logit(row + e);
-      if (x > -INFINITY) part += exp(static_cast<double>(x) - top);
-    }
-  const double total = sum64<32>(top, part);
+    for (int e = lane; e < a.E; e += 32) part += term64(load_logit(row + e), top);
+  const double total = sum64<32>(part);
   for (int e = lane; e < a.E; e += 32) keys[e] = key64(load_logit(row + e), top, total, a.bias, e, a.sigmoid);
   __syncwarp();
   unsigned bits = FULL;
@@ -199,11 +198,8 @@ __device__ __noinline__ int exact_places(const L* row, const RouteArgs& a, float
   const int rank = lane % LANES, base = lane - rank;
   double part = 0.0;
   if (!a.sigmoid)
-    for (int e = rank; e < a.E; e += LANES) {
-      const float x = load_logit(row + e);
-      if (x > -INFINITY) part += exp(static_cast<double>(x) - top);
-    }
-  const double total = sum64<LANES>(top, part);
+    for (int e = rank; e < a.E; e += LANES) part += term64(load_logit(row + e), top);
+  const double total = sum64<LANES>(part);
   const double mine = id >= 0 ? key64(load_logit(row + id), top, total, a.bias, id, a.sigmoid) : -INFINITY;
   int ahead = 0;
   for (int c = 0; c < most; ++c) {
@@ -313,7 +309,7 @@ select_experts_kernel(const L* logits, bool vectors, bool bias_vectors, RouteArg
     if (!LOGITS) {
       // errors of a key before its sum is rounded. sigmoid: exp's |x| 6e-8 + 2.4e-7 times s (1 - s), the reciprocal's 6e-8 s and the
       // sum 1 + exp's as much; softmax: exp's times exp(-|x|), its sum's and the reciprocal's, 4e-7 together, of the largest
-      const float inv = __fdividef(1.f, total);
+      const float inv = bad ? NAN : __fdividef(1.f, total);            // no key of a bad row compares
       slack = a.sigmoid ? 3e-7f : 1e-6f * inv;
       float b[PER];
       if (a.bias != nullptr) load_row<PER>(a.bias, first, a.E, bias_vectors, b);
@@ -598,6 +594,11 @@ template <int PER, bool WHOLE, class L> struct Spread {
 // A warp to a token. 65,537 x 512 bf16: sigmoid 22 us (67 MB written), softmax renormalised 25.5 (67 MB read too, for the largest logit), not
 // renormalised 33 (an exponential for each, kept in registers). 8,192 x 256 fp32, sigmoid: 4.3, of which a launch is half.
 constexpr float PICKS_NEAR = 20.f;
+__device__ __forceinline__ float max_or_nan(float x, float y) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x), "f"(y));
+  return m;
+}
 __device__ __forceinline__ float below(float x, float top) { return x == -INFINITY ? 0.f : exp_of(x - top); }
 enum { SIGMOID, SOFTMAX_RENORMALISED, SOFTMAX };
 constexpr int bwd_resident(int mode, int per) { return mode != SOFTMAX || per <= 4 ? 16 : per == 8 ? 12 : 10; }
@@ -617,7 +618,7 @@ select_experts_bwd_kernel(const L* logits, RouteArgs a, const int* ids, const fl
     if (MODE != SIGMOID) {
       Row::load(row, lane, a.E, v);
 #pragma unroll
-      for (int i = 0; i < PER; ++i) top = fmaxf(top, v[i]);
+      for (int i = 0; i < PER; ++i) top = max_or_nan(top, v[i]);
     }
     const bool in = pick && id >= 0 && id < a.E;
     const float d = in ? a.scale * dweights[static_cast<long long>(t) * a.k + lane] : 0.f;
@@ -628,8 +629,10 @@ select_experts_bwd_kernel(const L* logits, RouteArgs a, const int* ids, const fl
       s = sigmoid_score(x, other);
     } else {
       float base = warp_max32(x);
-      top = warp_max32(top);
-      if (MODE == SOFTMAX_RENORMALISED) others = !(base >= top - PICKS_NEAR);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = max_or_nan(top, __shfl_xor_sync(FULL, top, o));
+      const bool bad = !(top < INFINITY);        // a NaN or +inf in the row: scores, weights and gradients are NaN
+      if (MODE == SOFTMAX_RENORMALISED) others = bad || !(base >= top - PICKS_NEAR);
       if (others) {
         total = 0.f;
         if (MODE == SOFTMAX) {
@@ -644,7 +647,7 @@ select_experts_bwd_kernel(const L* logits, RouteArgs a, const int* ids, const fl
         total = fmaxf(warp_sum32(total), 1.f);
         base = top;
       }
-      s = x == -INFINITY ? 0.f : quotient(expf(x - base), total);
+      s = bad ? NAN : x == -INFINITY ? 0.f : quotient(expf(x - base), total);
     }
     float mine;                                  // dc_j s_j
     if (a.renormalize) {

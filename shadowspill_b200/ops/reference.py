@@ -338,8 +338,8 @@ def select_experts_bwd(logits, ids, dweights, scoring="softmax", renormalize=Tru
     if renormalize:
         total = c.sum(-1, keepdim=True) + 1e-20
         dc = (dc - (dc * c / total).sum(-1, keepdim=True)) / total
-    wide = torch.zeros_like(s).scatter_(1, at, dc)
-    dx = wide * s * (1 - s) if scoring == "sigmoid" else s * (wide - (dc * c).sum(-1, keepdim=True))
+    wide = torch.zeros_like(s).scatter_(1, at, dc * c * (1 - c) if scoring == "sigmoid" else dc)
+    dx = wide if scoring == "sigmoid" else s * (wide - (dc * c).sum(-1, keepdim=True))
     return dx.to(logits.dtype)
 
 

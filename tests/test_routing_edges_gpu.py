@@ -88,3 +88,38 @@ def test_gradient_of_softmax_picks_far_below_the_top(gap, renormalize, E, k, dty
     least = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
     allowed = 4 * score * size + left + torch.finfo(dtype).eps / 2 * want.abs() + 4 * k * low * dw.abs().sum(1, keepdim=True) + 2 * least
     assert bool(((got.double() - want).abs() <= allowed).all())
+
+
+@pytest.mark.parametrize("E,k,groups,keep", [(48, 3, 1, 1), (48, 8, 1, 1), (48, 6, 4, 2), (60, 6, 5, 2), (256, 5, 1, 1), (512, 10, 8, 3)])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_rows_with_nan_or_inf_follow_the_definition(E, k, groups, keep, bias, scoring, renormalize):
+    """A softmax with a NaN or +inf has no score that compares: the first experts are picked, with weights and gradients of NaN. Rows between
+    such rows, some with keys a few units in the last place apart, are what they are without them."""
+    nan, inf = float("nan"), float("inf")
+    x = _rand(64, E, seed=E)
+    x[1::4] = x[1::4, :1] + torch.randint(-4, 5, (16, E), generator=torch.Generator(device=DEV).manual_seed(2), device=DEV) * 2.0 ** -22
+    x[0, 5] = x[2, 0] = nan
+    x[4] = nan
+    x[6, 7], x[8, 3:6] = inf, inf
+    x[10], x[10, 9] = -inf, nan
+    x[12], x[12, 11] = -inf, inf
+    x[14, 1], x[14, 2] = nan, inf
+    x[16, :5], x[16, E - 1] = -inf, nan
+    bad = [0, 2, 4, 6, 8, 10, 12, 14, 16]
+    b = _rand(E, seed=4) * 0.1 if bias else None
+    for dtype in (torch.float32, torch.bfloat16):
+        y = x.to(dtype)
+        ids, w, counts = routing.select_experts(y, k, scoring=scoring, bias=b, groups=groups, keep_groups=keep, renormalize=renormalize)
+        want = R.select_experts(y, k, scoring, b, groups, keep, renormalize)
+        assert torch.equal(ids, want[0]) and torch.equal(counts, want[2])
+        assert torch.equal(torch.isnan(w), torch.isnan(want[1]))
+        dw = _rand(64, k, seed=5)
+        got = routing.select_experts_bwd(y, ids, dw, scoring=scoring, renormalize=renormalize)
+        ref = R.select_experts_bwd(y.double(), ids, dw, scoring, renormalize)
+        assert torch.equal(torch.isnan(got), torch.isnan(ref))
+        if scoring == "softmax":
+            if bias or groups > 1:
+                assert torch.equal(ids[bad], torch.arange(k, dtype=torch.int32, device=DEV).expand(9, k))
+            assert bool(torch.isnan(w[bad]).all()) and bool(torch.isnan(got[bad]).all())
