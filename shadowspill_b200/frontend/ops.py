@@ -20,6 +20,7 @@ import torch
 from torch.library import custom_op
 
 from ..ops import functional as F
+from ..ops import reference
 from ..ops import token_head
 
 Tensor = torch.Tensor
@@ -815,9 +816,16 @@ sparse_latent_attention.register_autograd(_sla_bwd, setup_context=_sla_setup)
 @custom_op("ss::select_experts", mutates_args=())
 def select_experts(logits: Tensor, bias: Tensor, k: int, sigmoid: bool, groups: int, keep_groups: int, renorm: bool,
                    scale: float) -> tuple[Tensor, Tensor]:
-    """``routing.select_experts`` by rows: the picks and their weights (``bias`` only selects and is never trained)."""
+    """``routing.select_experts`` by rows: the picks and their weights (``bias`` only selects and is never trained). Without the kernels
+    there is no bound on the experts."""
     from ..ops import routing
-    ids, wts, _ = routing.select_experts(logits, k, scoring="sigmoid" if sigmoid else "softmax", bias=bias, groups=groups,
+    scoring = "sigmoid" if sigmoid else "softmax"
+    if not F._cuda(logits):
+        if not 1 <= k <= keep_groups * (logits.shape[1] // groups):
+            raise ValueError(f"cannot pick {k} of {keep_groups * (logits.shape[1] // groups)} experts")
+        ids, wts, _ = reference.select_experts(logits, k, scoring, bias, groups, keep_groups, renorm, scale)
+        return ids, wts
+    ids, wts, _ = routing.select_experts(logits, k, scoring=scoring, bias=bias, groups=groups,
                                          keep_groups=keep_groups, renormalize=renorm, scale=scale)
     return ids, wts
 
@@ -830,7 +838,10 @@ def _(logits, bias, k, sigmoid, groups, keep_groups, renorm, scale):
 @custom_op("ss::select_experts_bwd", mutates_args=())
 def select_experts_bwd(logits: Tensor, ids: Tensor, dwts: Tensor, sigmoid: bool, renorm: bool, scale: float) -> Tensor:
     from ..ops import routing
-    return routing.select_experts_bwd(logits, ids, _c(dwts), scoring="sigmoid" if sigmoid else "softmax", renormalize=renorm, scale=scale)
+    scoring = "sigmoid" if sigmoid else "softmax"
+    if not F._cuda(logits):
+        return reference.select_experts_bwd(logits, ids, dwts, scoring, renorm, scale)
+    return routing.select_experts_bwd(logits, ids, _c(dwts), scoring=scoring, renormalize=renorm, scale=scale)
 
 
 @select_experts_bwd.register_fake

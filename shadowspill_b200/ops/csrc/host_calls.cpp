@@ -363,7 +363,7 @@ PyObject* select_experts(PyObject*, PyObject* const* v, Py_ssize_t n) {
     const bool f32 = logits_rows(x);
     void* stream = stream_of(x);
     const int64_t T = x.size(0), E = x.size(1), k = integer(v[1]), sigmoid = integer(v[2]), groups = integer(v[4]), keep = integer(v[5]);
-    want((sigmoid == 0 || sigmoid == 1) && E >= 1 && E <= 512 && k >= 1 && k <= 32 && groups >= 1 && groups <= 32 && E % groups == 0 &&
+    want((sigmoid == 0 || sigmoid == 1) && E >= 1 && E <= 512 && k >= 1 && groups >= 1 && groups <= 32 && E % groups == 0 &&
          keep >= 1 && keep <= groups && k <= keep * (E / groups));
     const float* bias = floats(v[3], E, x);
     const auto options = x.options().requires_grad(false);
@@ -386,7 +386,7 @@ PyObject* select_experts_bwd(PyObject*, PyObject* const* v, Py_ssize_t n) {
     contiguous(dw, at::kFloat);
     want(ids.dim() == 2 && dw.sizes() == ids.sizes() && ids.size(0) == x.size(0) && on(ids, x) && on(dw, x));
     const int64_t T = x.size(0), E = x.size(1), k = ids.size(1), sigmoid = integer(v[3]);
-    want((sigmoid == 0 || sigmoid == 1) && E >= 1 && E <= 512 && k >= 1 && k <= 32 && k <= E);
+    want((sigmoid == 0 || sigmoid == 1) && E >= 1 && E <= 512 && k >= 1 && k <= E);
     at::Tensor out = empty({T, E}, x.options().requires_grad(false));
     launch(SELECT_BWD, ss_select_experts_bwd, x.data_ptr(), !f32, pitch(x), static_cast<const int*>(ids.data_ptr()),
            static_cast<const float*>(dw.data_ptr()), T, E, k, sigmoid, v[4] == Py_True, static_cast<float>(number(v[5])),

@@ -23,7 +23,7 @@ namespace ss {
 namespace {
 
 constexpr int RT_THREADS = 128, RT_WARPS = RT_THREADS / 32;
-constexpr int RT_MAX_E = 512, RT_MAX_K = 32, RT_MAX_GROUPS = 32;
+constexpr int RT_MAX_E = 512, RT_MAX_GROUPS = 32;
 constexpr unsigned FULL = 0xffffffffu;
 
 __device__ __forceinline__ float load_logit(const float* p) { return *p; }
@@ -137,22 +137,31 @@ __device__ __forceinline__ double sum64(double part) {
   for (int o = LANES / 2; o > 0; o >>= 1) part += __shfl_xor_sync(FULL, part, o);
   return part == 0.0 ? 1.0 : part;
 }
+__device__ __forceinline__ double score64(float x, float top, double total, bool sigmoid) {
+  return sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(x))) : term64(x, top) / total;
+}
 __device__ __forceinline__ double key64(float x, float top, double total, const float* bias, int e, bool sigmoid) {
-  double v = sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(x))) : term64(x, top) / total;
+  double v = score64(x, top, total, sigmoid);
   if (bias != nullptr) v += bias[e];
   return v == v ? v : -INFINITY;
 }
 
-// All keys of a row in 64 bits into shared memory, by a whole warp, and the groups that stay, as bits.
+// A row's largest logit and its softmax's sum in 64 bits, by a whole warp.
 template <class L>
-__device__ __noinline__ unsigned exact_keys(const L* row, const RouteArgs& a, double* keys, int lane) {
-  float top = -INFINITY;
+__device__ __forceinline__ double whole_sum64(const L* row, const RouteArgs& a, int lane, float& top) {
+  top = -INFINITY;
   for (int e = lane; e < a.E; e += 32) top = fmaxf(top, load_logit(row + e));
   top = warp_max32(top);
   double part = 0.0;
   if (!a.sigmoid)
     for (int e = lane; e < a.E; e += 32) part += term64(load_logit(row + e), top);
-  const double total = sum64<32>(part);
+  return sum64<32>(part);
+}
+// All keys of a row in 64 bits into shared memory, by a whole warp, and the groups that stay, as bits.
+template <class L>
+__device__ __noinline__ unsigned exact_keys(const L* row, const RouteArgs& a, double* keys, int lane) {
+  float top;
+  const double total = whole_sum64(row, a, lane, top);
   for (int e = lane; e < a.E; e += 32) keys[e] = key64(load_logit(row + e), top, total, a.bias, e, a.sigmoid);
   __syncwarp();
   unsigned bits = FULL;
@@ -164,27 +173,36 @@ __device__ __noinline__ unsigned exact_keys(const L* row, const RouteArgs& a, do
   return bits;
 }
 
-// The picks among those keys; lane j returns the j-th.
-__device__ __noinline__ int picks_exact(const RouteArgs& a, unsigned bits, const unsigned char* group_of, double* keys, int lane) {
+// Keys of the groups that do not stay become -inf.
+__device__ __forceinline__ void drop_groups(const RouteArgs& a, unsigned bits, const unsigned char* group_of, double* keys, int lane) {
   for (int e = lane; e < a.E; e += 32)
     if (!((bits >> group_of[e]) & 1)) keys[e] = -INFINITY;
   __syncwarp();
-  unsigned taken = 0;                            // this lane's experts that are picked, by place
+}
+// The largest key that is not picked yet, by a whole warp; `taken`: this lane's experts that are, by place.
+__device__ __forceinline__ int next_pick(const RouteArgs& a, const double* keys, int lane, unsigned& taken) {
+  double best = -INFINITY;
+  int at = INT_MAX;
+  for (int i = 0; lane + 32 * i < a.E; ++i) {
+    const int e = lane + 32 * i;
+    if (!((taken >> i) & 1) && (at == INT_MAX || keys[e] > best)) { best = keys[e]; at = e; }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const double ob = __shfl_xor_sync(FULL, best, o);
+    const int oa = __shfl_xor_sync(FULL, at, o);
+    if (oa != INT_MAX && (at == INT_MAX || ob > best || (ob == best && oa < at))) { best = ob; at = oa; }
+  }
+  if ((at & 31) == lane) taken |= 1u << (at >> 5);
+  return at;
+}
+// The picks among those keys; lane j returns the j-th.
+__device__ __noinline__ int picks_exact(const RouteArgs& a, unsigned bits, const unsigned char* group_of, double* keys, int lane) {
+  drop_groups(a, bits, group_of, keys, lane);
+  unsigned taken = 0;
   int mine = 0;
   for (int j = 0; j < a.k; ++j) {
-    double best = -INFINITY;
-    int at = INT_MAX;
-    for (int i = 0; lane + 32 * i < a.E; ++i) {
-      const int e = lane + 32 * i;
-      if (!((taken >> i) & 1) && (at == INT_MAX || keys[e] > best)) { best = keys[e]; at = e; }
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const double ob = __shfl_xor_sync(FULL, best, o);
-      const int oa = __shfl_xor_sync(FULL, at, o);
-      if (oa != INT_MAX && (at == INT_MAX || ob > best || (ob == best && oa < at))) { best = ob; at = oa; }
-    }
-    if ((at & 31) == lane) taken |= 1u << (at >> 5);
+    const int at = next_pick(a, keys, lane, taken);
     if (lane == j) mine = at;
   }
   __syncwarp();
@@ -552,6 +570,57 @@ select_experts_kernel(const L* logits, bool vectors, bool bias_vectors, RouteArg
   }
 }
 
+// More picks than a warp has lanes: all keys in 64 bits, picked one by one, a warp to a token. 8,192 tokens, 40 of 256 experts by sigmoid: 126 us.
+template <class L>
+__global__ void __launch_bounds__(RT_THREADS)
+select_many_kernel(const L* logits, RouteArgs a, int* ids, float* weights, int* counts) {
+  chain_wait();
+  chain_release();
+  __shared__ int hist[RT_MAX_E];
+  __shared__ unsigned char group_of[RT_MAX_E];
+  extern __shared__ double warp_keys[];          // E to a warp; then the warps' picks
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, size = a.E / a.groups;
+  double* const keys = warp_keys + warp * a.E;
+  int* const picks = reinterpret_cast<int*>(warp_keys + RT_WARPS * a.E) + warp * a.k;
+  for (int e = threadIdx.x; e < a.E; e += RT_THREADS) {
+    hist[e] = 0;
+    group_of[e] = static_cast<unsigned char>(e / size);
+  }
+  __syncthreads();
+  for (int t = blockIdx.x * RT_WARPS + warp; t < a.T; t += gridDim.x * RT_WARPS) {
+    const L* row = logits + static_cast<long long>(t) * a.ld;
+    float top;
+    const double total = whole_sum64(row, a, lane, top);
+    if (a.bias == nullptr && a.groups == 1) {    // the logits themselves, as above
+      for (int e = lane; e < a.E; e += 32) keys[e] = fmaxf(load_logit(row + e), -INFINITY);
+      __syncwarp();
+    } else {
+      drop_groups(a, exact_keys(row, a, keys, lane), group_of, keys, lane);
+    }
+    unsigned taken = 0;
+    for (int j = 0; j < a.k; ++j) {
+      const int at = next_pick(a, keys, lane, taken);
+      if (lane == 0) picks[j] = at;
+    }
+    __syncwarp();
+    double sum = 0.0;
+    for (int j = lane; j < a.k; j += 32) sum += score64(load_logit(row + picks[j]), top, total, a.sigmoid);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL, sum, o);
+    const double by = a.renormalize ? a.scale / (sum + 1e-20) : a.scale;
+    for (int j = lane; j < a.k; j += 32) {
+      const int e = picks[j];
+      ids[static_cast<long long>(t) * a.k + j] = e;
+      weights[static_cast<long long>(t) * a.k + j] = static_cast<float>(score64(load_logit(row + e), top, total, a.sigmoid) * by);
+      atomicAdd(&hist[e], 1);
+    }
+    __syncwarp();                                // keys and picks of the next token come into the same place
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.E; e += RT_THREADS)
+    if (hist[e]) atomicAdd(counts + e, hist[e]);
+}
+
 __global__ void clear_counts_kernel(int* counts, int E) {
   chain_wait();
   chain_release();
@@ -602,33 +671,44 @@ __device__ __forceinline__ float max_or_nan(float x, float y) {
 __device__ __forceinline__ float below(float x, float top) { return x == -INFINITY ? 0.f : exp_of(x - top); }
 enum { SIGMOID, SOFTMAX_RENORMALISED, SOFTMAX };
 constexpr int bwd_resident(int mode, int per) { return mode != SOFTMAX || per <= 4 ? 16 : per == 8 ? 12 : 10; }
-template <int MODE, int PER, bool WHOLE, class L>
-__global__ void __launch_bounds__(RT_THREADS, bwd_resident(MODE, PER))
+// MANY: more picks than lanes, every 32nd to a lane.
+template <int MODE, int PER, bool WHOLE, bool MANY, class L>
+__global__ void __launch_bounds__(RT_THREADS, MANY ? 4 : bwd_resident(MODE, PER))
 select_experts_bwd_kernel(const L* logits, RouteArgs a, const int* ids, const float* dweights, L* dlogits) {
   using Row = Spread<PER, WHOLE, L>;
+  constexpr int OWN = MANY ? RT_MAX_E / 32 : 1;
   chain_wait();
   chain_release();
   const int lane = threadIdx.x & 31;
   for (int t = blockIdx.x * RT_WARPS + (threadIdx.x >> 5); t < a.T; t += gridDim.x * RT_WARPS) {
     const L* row = logits + static_cast<long long>(t) * a.ld;
     L* out = dlogits + static_cast<long long>(t) * a.E;
-    const bool pick = lane < a.k;
-    const int id = pick ? ids[static_cast<long long>(t) * a.k + lane] : 0;
+    int id[OWN];                                 // -1: none
+    float d[OWN], x[OWN], s[OWN], other[OWN];
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) id[i] = lane + 32 * i < a.k ? ids[static_cast<long long>(t) * a.k + lane + 32 * i] : -1;
     float v[PER], top = -INFINITY;
     if (MODE != SIGMOID) {
       Row::load(row, lane, a.E, v);
 #pragma unroll
       for (int i = 0; i < PER; ++i) top = max_or_nan(top, v[i]);
     }
-    const bool in = pick && id >= 0 && id < a.E;
-    const float d = in ? a.scale * dweights[static_cast<long long>(t) * a.k + lane] : 0.f;
-    const float x = in ? load_logit(row + id) : -INFINITY;
-    float total = 1.f, s, other = 0.f, inner = 0.f;
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      if (id[i] >= a.E) id[i] = -1;
+      d[i] = id[i] >= 0 ? a.scale * dweights[static_cast<long long>(t) * a.k + lane + 32 * i] : 0.f;
+      x[i] = id[i] >= 0 ? load_logit(row + id[i]) : -INFINITY;
+    }
+    float total = 1.f, inner = 0.f;
     bool others = MODE == SOFTMAX;               // do experts that were not picked have gradients?
     if (MODE == SIGMOID) {
-      s = sigmoid_score(x, other);
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) s[i] = sigmoid_score(x[i], other[i]);
     } else {
-      float base = warp_max32(x);
+      float base = x[0];
+#pragma unroll
+      for (int i = 1; i < OWN; ++i) base = fmaxf(base, x[i]);
+      base = warp_max32(base);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = max_or_nan(top, __shfl_xor_sync(FULL, top, o));
       const bool bad = !(top < INFINITY);        // a NaN or +inf in the row: scores, weights and gradients are NaN
@@ -647,16 +727,31 @@ select_experts_bwd_kernel(const L* logits, RouteArgs a, const int* ids, const fl
         total = fmaxf(warp_sum32(total), 1.f);
         base = top;
       }
-      s = bad ? NAN : x == -INFINITY ? 0.f : quotient(expf(x - base), total);
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) s[i] = bad ? NAN : x[i] == -INFINITY ? 0.f : quotient(expf(x[i] - base), total);
     }
-    float mine;                                  // dc_j s_j
+    float mine[OWN], part = 0.f;                 // dc_j s_j
     if (a.renormalize) {
-      const float sum = warp_sum32(s) + 1e-20f, u = quotient(s, sum), mean = warp_sum32(d * u);
-      mine = (d - mean) * u;
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) part += s[i];
+      const float sum = warp_sum32(part) + 1e-20f;
+      part = 0.f;
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) {
+        mine[i] = quotient(s[i], sum);
+        part += d[i] * mine[i];
+      }
+      const float mean = warp_sum32(part);
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) mine[i] *= d[i] - mean;
       if (others) inner = mean * quotient(1e-20f, sum);
     } else {
-      mine = d * s;
-      if (MODE == SOFTMAX) inner = warp_sum32(mine);
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) {
+        mine[i] = d[i] * s[i];
+        part += mine[i];
+      }
+      if (MODE == SOFTMAX) inner = warp_sum32(part);
     }
     const float each = others ? -quotient(inner, total) : 0.f;
     if (MODE == SOFTMAX) {
@@ -670,12 +765,14 @@ select_experts_bwd_kernel(const L* logits, RouteArgs a, const int* ids, const fl
       Row::store(out, lane, a.E, zero);
     }
     __syncwarp();                                // the picks overwrite what another lane wrote above
-    if (in) store_logit(out + id, MODE == SIGMOID ? mine * other : mine - s * inner);
+#pragma unroll
+    for (int i = 0; i < OWN; ++i)
+      if (id[i] >= 0) store_logit(out + id[i], MODE == SIGMOID ? mine[i] * other[i] : mine[i] - s[i] * inner);
   }
 }
 
 bool fits(const RouteArgs& a) {
-  return a.T >= 0 && a.T <= 0x7fff0000 && a.E >= 1 && a.E <= RT_MAX_E && a.k >= 1 && a.k <= RT_MAX_K && a.k <= a.E && a.groups >= 1 &&
+  return a.T >= 0 && a.T <= 0x7fff0000 && a.E >= 1 && a.E <= RT_MAX_E && a.k >= 1 && a.k <= a.E && a.groups >= 1 &&
          a.groups <= RT_MAX_GROUPS && a.E % a.groups == 0 && a.keep >= 1 && a.keep <= a.groups &&
          a.k <= a.keep * (a.E / a.groups) && a.ld >= a.E;
 }
@@ -692,6 +789,14 @@ int ss_select_experts(const void* logits, int bf16_logits, long long ld, const f
   const RouteArgs a{T, E, k, groups, keep_groups, sigmoid, renormalize, ld, scale, bias};
   if (!fits(a)) return -2;
   cudaStream_t s = (cudaStream_t)stream;
+  if (k > 32) {
+    const int blocks = (T + RT_WARPS - 1) / RT_WARPS, grid = blocks < 1 ? 1 : blocks < 148 * 8 ? blocks : 148 * 8;
+    const size_t smem = RT_WARPS * (sizeof(double) * E + sizeof(int) * k);
+    launch_chained(clear_counts_kernel, 1, 128, 0, s, counts, E);
+    if (bf16_logits) launch_chained(select_many_kernel<__nv_bfloat16>, grid, RT_THREADS, smem, s, (const __nv_bfloat16*)logits, a, ids, weights, counts);
+    else launch_chained(select_many_kernel<float>, grid, RT_THREADS, smem, s, (const float*)logits, a, ids, weights, counts);
+    return (int)cudaGetLastError();
+  }
   const bool plain = bias == nullptr && groups == 1;
   // Half a warp to a token where the candidates are hardly ever more than its lanes: a token too many in twenty at k = 8 of 16
   // costs little where logits are compared, but what is doubtful of it is settled over a whole row, which the launch waits for (8,192
@@ -732,14 +837,17 @@ int ss_select_experts_bwd(const void* logits, int bf16_logits, long long ld, con
   if (!fits(a)) return -2;
   if (T == 0) return 0;
   const int per = (E + 31) / 32, blocks = (T + RT_WARPS - 1) / RT_WARPS;
-  auto go = [&](auto mode, auto n, auto whole, auto* x, auto* out) {
-    using X = std::remove_pointer_t<decltype(out)>;
-    const int most = 148 * bwd_resident(mode, n), grid = blocks < most ? blocks : most;
-    launch_chained(select_experts_bwd_kernel<decltype(mode)::value, decltype(n)::value, decltype(whole)::value, X>, grid, RT_THREADS, 0,
-                   (cudaStream_t)stream, x, a, ids, dweights, out);
+  auto launch = [&](auto kern, int resident, auto* x, auto* out) {
+    launch_chained(kern, blocks < 148 * resident ? blocks : 148 * resident, RT_THREADS, 0, (cudaStream_t)stream, x, a, ids, dweights, out);
     return (int)cudaGetLastError();
   };
+  auto go = [&](auto mode, auto n, auto whole, auto* x, auto* out) {
+    constexpr int M = decltype(mode)::value, N = decltype(n)::value;
+    using X = std::remove_pointer_t<decltype(out)>;
+    return launch(select_experts_bwd_kernel<M, N, decltype(whole)::value, false, X>, bwd_resident(M, N), x, out);
+  };
   auto by_length = [&](auto mode, auto whole, auto* x, auto* out) {
+    if (k > 32) return launch(select_experts_bwd_kernel<decltype(mode)::value, 16, false, true, std::remove_pointer_t<decltype(out)>>, 4, x, out);
     if (per <= 2) return go(mode, std::integral_constant<int, 2>(), whole, x, out);
     if (per <= 4) return go(mode, std::integral_constant<int, 4>(), whole, x, out);
     if (per <= 8) return go(mode, std::integral_constant<int, 8>(), whole, x, out);

@@ -17,7 +17,7 @@ _P, _I, _L, _F = _lib.c_p, _lib.c_int, _lib.c_ll, _lib.c_f
 _lib.register("ss_select_experts", [_P, _I, _L, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P, _P])
 _lib.register("ss_select_experts_bwd", [_P, _I, _L, _P, _P, _I, _I, _I, _I, _I, _F, _P, _P])
 
-MAX_EXPERTS, MAX_K, MAX_GROUPS = 512, 32, 32          # as the kernels have them
+MAX_EXPERTS, MAX_GROUPS = 512, 32                     # as the kernels have them
 _SIGMOID = {"softmax": 0, "sigmoid": 1}
 
 
@@ -29,8 +29,8 @@ def _check(logits, k, scoring, groups=1, keep_groups=1):
         raise ValueError(f"unknown scoring {scoring!r}; known: {tuple(_SIGMOID)}")
     if not (1 <= groups <= MAX_GROUPS and E % groups == 0 and 1 <= keep_groups <= groups):
         raise ValueError(f"{E} experts do not fall into {groups} groups of which {keep_groups} are kept")
-    if not (1 <= k <= MAX_K and E <= MAX_EXPERTS and k <= keep_groups * (E // groups)):
-        raise ValueError(f"cannot pick {k} of {keep_groups * (E // groups)} experts (at most {MAX_K} of {MAX_EXPERTS})")
+    if not (1 <= k <= keep_groups * (E // groups) and E <= MAX_EXPERTS):
+        raise ValueError(f"cannot pick {k} of {keep_groups * (E // groups)} experts (of at most {MAX_EXPERTS})")
 
 
 def select_experts(logits: torch.Tensor, k: int, *, scoring: str = "softmax", bias: torch.Tensor | None = None,
@@ -41,7 +41,8 @@ def select_experts(logits: torch.Tensor, k: int, *, scoring: str = "softmax", bi
     largest sum highest, in decreasing order, ties to the lowest index; they are those of keys in 64 bits. Experts whose key is
     -inf or NaN come last, so that the ids of a token are always ``k`` different experts. The weights are the picks' scores
     (without the bias), divided by their sum (+ 1e-20) if ``renormalize``, times ``scale``; a token whose logits are all -inf
-    gets weights of zero under softmax, one with a NaN or +inf gets NaN."""
+    gets weights of zero under softmax, one with a NaN or +inf gets NaN. At most 512 experts; ``k`` has no bound of its own (above 32 the
+    picks are made one by one in 64 bits, five times as long)."""
     host = F._host(logits)
     if host is not None:
         got = host.select_experts(logits, k, _SIGMOID.get(scoring, -1), bias, groups, keep_groups, bool(renormalize), scale)

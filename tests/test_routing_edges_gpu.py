@@ -123,3 +123,81 @@ def test_rows_with_nan_or_inf_follow_the_definition(E, k, groups, keep, bias, sc
             if bias or groups > 1:
                 assert torch.equal(ids[bad], torch.arange(k, dtype=torch.int32, device=DEV).expand(9, k))
             assert bool(torch.isnan(w[bad]).all()) and bool(torch.isnan(got[bad]).all())
+
+
+# relative error of a weight of 33 to 512 picks: exponentials off by 2 steps and their argument's rounding (up to 16), twice; sums of 16 terms
+# to a lane and five levels, twice; two quotients
+MANY = (2 * (2 + 8) + 2 * 21 + 4) * STEP
+
+
+@pytest.mark.parametrize("T,E,k,groups,keep", [(1, 33, 33, 1, 1), (50, 64, 40, 1, 1), (70, 512, 512, 1, 1), (9, 96, 48, 3, 2), (2500, 256, 33, 8, 5),
+                                              (30, 511, 100, 1, 1), (0, 64, 40, 1, 1)])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_more_picks_than_a_warp_has_lanes(T, E, k, groups, keep, bias, scoring, dtype):
+    x, b = (_rand(T, E, seed=T) * 1.5).to(dtype), _rand(E, seed=3) * 0.1 if bias else None
+    dw = _rand(T, k, seed=8)
+    for renormalize in (True, False):
+        ids, w, counts = routing.select_experts(x, k, scoring=scoring, bias=b, groups=groups, keep_groups=keep, renormalize=renormalize, scale=2.5)
+        want = R.select_experts(x, k, scoring, b, groups, keep, renormalize, 2.5)
+        assert torch.equal(ids, want[0]) and torch.equal(counts, want[2])
+        assert bool(((w - want[1]).abs() <= STEP * want[1]).all())               # rounded once, in either
+        got = routing.select_experts_bwd(x, ids, dw, scoring=scoring, renormalize=renormalize, scale=2.5)
+        ref = R.select_experts_bwd(x.double(), ids, dw, scoring, renormalize, 2.5)
+        s = R.expert_scores(x.double(), scoring)
+        total = s.gather(1, ids.long()).sum(1, keepdim=True) if renormalize else 1.0
+        most = 2.5 * dw.abs().amax(1, keepdim=True)                            # of the terms that may cancel
+        size = most * s / total * (2 if renormalize else 1) + (0 if scoring == "sigmoid" else most * s / total)
+        assert bool(((got - ref).abs() <= 2 * MANY * size + torch.finfo(dtype).eps / 2 * ref.abs()).all())
+
+
+def test_many_picks_of_ties_masks_and_bad_rows():
+    nan, inf = float("nan"), float("inf")
+    g = torch.Generator(device=DEV).manual_seed(5)
+    x = torch.randint(-2, 3, (64, 80), generator=g, device=DEV).float() * 0.5
+    x[0], x[1, 3:], x[2, 5], x[3, 7], x[4] = -inf, -inf, nan, inf, nan
+    for b in (None, torch.zeros(80, device=DEV)):
+        for scoring in ("softmax", "sigmoid"):
+            ids, w, counts = routing.select_experts(x, 50, scoring=scoring, bias=b)
+            want = R.select_experts(x, 50, scoring, b)
+            assert torch.equal(ids, want[0]) and torch.equal(counts, want[2]) and torch.equal(torch.isnan(w), torch.isnan(want[1]))
+            got = routing.select_experts_bwd(x, ids, w.nan_to_num(), scoring=scoring)
+            ref = R.select_experts_bwd(x.double(), ids, w.nan_to_num(), scoring)
+            assert torch.equal(torch.isnan(got), torch.isnan(ref))
+
+
+def test_many_picks_captured_and_on_another_stream():
+    x, dw = _rand(600, 64, seed=1), _rand(600, 40, seed=2)
+    routing.select_experts(x, 40)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ids, w, counts = routing.select_experts(x, 40, scoring="sigmoid")
+        grad = routing.select_experts_bwd(x, ids, dw, scoring="sigmoid")
+    x.copy_(_rand(600, 64, seed=11))
+    graph.replay()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = routing.select_experts(x, 40, scoring="sigmoid")
+        want_grad = routing.select_experts_bwd(x, want[0], dw, scoring="sigmoid")
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip((ids, w, counts, grad), (*want, want_grad)))
+
+
+def test_a_layer_of_more_picks_than_lanes():
+    """Picks into the experts' products, forward and backward, against the tensor-operation form."""
+    import shadowspill_b200.frontend.ops as ops
+    T, D, Fw, E, k = 64, 128, 128, 48, 40
+    h, w13, w2 = _rand(T, D, seed=1).bfloat16(), (_rand(E, 2 * Fw, D, seed=2) * 0.1).bfloat16(), (_rand(E, D, Fw, seed=3) * 0.1).bfloat16()
+    logits, bias = _rand(T, E, seed=4), _rand(E, seed=5) * 0.1
+    ids, w = torch.ops.ss.select_experts(logits, bias, k, True, 1, 1, True, 2.5)
+    out, up = torch.ops.ss.moe_experts_routed(h, ids, w, w13, w2), _rand(T, D, seed=6).bfloat16()
+    grads = torch.ops.ss.moe_experts_routed_bwd(h, ids, w, w13, w2, up, True)        # as exported stages call it
+    ref = [t.double().requires_grad_(True) for t in (h, w, w13, w2)]
+    want = ops._moe_routed_torch(ref[0], ids, *ref[1:])
+    want.backward(up.double())
+    # activations, products and their gradients are stored in bf16, four of them in a chain, each off by 2^-8 of its value
+    for got, exact in ((out, want), *((a, b.grad) for a, b in zip(grads, ref))):
+        assert float((got.double() - exact.detach()).norm()) <= 4 * 2.0 ** -8 * float(exact.detach().norm())

@@ -1,0 +1,35 @@
+"""Expert selection, preference objective and 8-bit AdamW on the CPU: calls at the edges of what they take."""
+import pytest
+import torch
+
+from shadowspill_b200.ops import reference as R
+
+
+def _rand(*shape, seed=0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed))
+
+
+@pytest.mark.parametrize("E,k", [(600, 3), (600, 40), (64, 33), (40, 40)])
+@pytest.mark.parametrize("sigmoid", [True, False])
+def test_layers_of_any_number_of_experts_route_on_the_cpu(E, k, sigmoid):
+    import shadowspill_b200.frontend.ops  # noqa: F401
+    x, bias, up = _rand(9, E).requires_grad_(True), _rand(E, seed=1) * 0.1, _rand(9, k, seed=2)
+    ids, w = torch.ops.ss.select_experts(x, bias, k, sigmoid, 1, 1, True, 1.5)
+    y = x.detach().double().requires_grad_(True)
+    s = torch.sigmoid(y) if sigmoid else torch.softmax(y, 1)
+    assert torch.equal(ids.long(), torch.sort(s + bias.double(), dim=1, descending=True, stable=True).indices[:, :k])
+    c = s.gather(1, ids.long())
+    want = 1.5 * c / (c.sum(1, keepdim=True) + 1e-20)
+    (w * up).sum().backward()
+    (want * up.double()).sum().backward()
+    # weights and gradients are formed in 64 bits and rounded once, but for fp32 weights in the sum above, which no gradient sees
+    assert bool(((w.double() - want).abs() <= 2.0 ** -24 * want).all())
+    assert bool(((x.grad.double() - y.grad).abs() <= 2.0 ** -23 * y.grad.abs() + 1e-12).all())
+
+
+def test_more_picks_than_experts_are_refused_on_the_cpu():
+    import shadowspill_b200.frontend.ops  # noqa: F401
+    for k, groups, keep in ((9, 1, 1), (0, 1, 1), (5, 4, 2)):
+        with pytest.raises(ValueError):
+            torch.ops.ss.select_experts(_rand(3, 8), torch.zeros(8), k, True, groups, keep, True, 1.0)
+    assert R.select_experts(_rand(3, 8), 8)[0].shape == (3, 8)
