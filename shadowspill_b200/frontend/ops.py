@@ -863,13 +863,6 @@ select_experts.register_autograd(_select_bwd, setup_context=_select_setup)
 
 
 # ------------------------------------------------------------------------ routed experts, routing given
-def _counts(ids: Tensor, E: int) -> Tensor:
-    """How often each expert was picked, without a word to the host (``bincount`` waits for the largest pick)."""
-    flat = ids.reshape(-1).long()
-    return torch.zeros(E, dtype=torch.int32, device=ids.device).index_add_(
-        0, flat, torch.ones(1, dtype=torch.int32, device=ids.device).expand(flat.numel()))
-
-
 def _moe_routed_torch(h: Tensor, ids: Tensor, wts: Tensor, w13: Tensor, w2: Tensor) -> Tensor:
     """Top-k SwiGLU experts with the routing decided outside (``ids`` [T, k], ``wts`` [T, k]): the
     form for routers that are not a softmax (sigmoid scores with a selection-only bias)."""
@@ -897,8 +890,7 @@ def _moe_routed_torch(h: Tensor, ids: Tensor, wts: Tensor, w13: Tensor, w2: Tens
 def _moe_routed_cuda(h, ids, wts, w13, w2, sink):
     from ..models import autograd_ops as A
     from ..ops import moe as moe_ops
-    counts = _counts(ids, w13.shape[0])
-    lay = moe_ops.Layout(ids.to(torch.int32).contiguous(), counts)
+    lay = moe_ops.Layout(*moe_ops.counted(ids, w13.shape[0]))
     xs = A.expert_gather(h, lay)
     ys = A.grouped_linear(A.swiglu(A.grouped_linear(xs, w13, lay, sink, "w13")), w2, lay, sink, "w2")
     return A.expert_combine(ys, wts.float().contiguous(), lay)
@@ -983,8 +975,7 @@ def _moe_routed_lora_torch(h, ids, wts, w13, w2, a13, b13, a2, b2, scale: float)
 def _moe_routed_lora_cuda(h, ids, wts, w13, w2, a13, b13, a2, b2, scale: float, sink):
     from ..models import autograd_ops as A
     from ..ops import moe as moe_ops
-    counts = _counts(ids, w13.shape[0])
-    lay = moe_ops.Layout(ids.to(torch.int32).contiguous(), counts)
+    lay = moe_ops.Layout(*moe_ops.counted(ids, w13.shape[0]))
     xs = A.expert_gather(h, lay)
 
     def bank(x, w, a, b, an, bn):

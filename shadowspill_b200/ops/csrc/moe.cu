@@ -3,6 +3,7 @@
 //   ss_moe_route      per token: top-k over the router logits, softmax over the
 //                     selected logits (renormalised) or over all experts, and a
 //                     per-expert histogram -- one warp per token, no sorting pass
+//   ss_moe_count      per-expert histogram of picks made elsewhere, those of no expert reported
 //   ss_moe_layout     expert segments padded to 128 rows (so a GEMM tile never
 //                     straddles two experts), the expert of every 128-row tile,
 //                     and a destination row for every (token, slot) assignment
@@ -25,6 +26,8 @@
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
+
+#include "sm100_ptx.cuh"
 
 namespace ss {
 
@@ -147,6 +150,32 @@ moe_route_bwd_kernel(const float* __restrict__ logits, long long ld, const int* 
   }
   __syncwarp();                                // the picks overwrite what another lane wrote above
   if (lane < k) out[id] = w * (dw - inner);
+}
+
+// The picks of a routing that was made elsewhere: how often each expert is among them, and the picks for the layout, which indexes by them. One
+// that names no expert is reported in the status word and goes to expert 0. 32,768 picks of 64 experts: 4 us.
+constexpr int COUNT_THREADS = 256, COUNT_PER_THREAD = 4;
+__global__ void __launch_bounds__(COUNT_THREADS)
+moe_count_kernel(const int* __restrict__ ids, long long n, int E, int* __restrict__ counts, int* __restrict__ picks, int* status) {
+  __shared__ int hist[MOE_MAX_E];
+  for (int e = threadIdx.x; e < E; e += COUNT_THREADS) hist[e] = 0;
+  __syncthreads();
+  const long long i0 = blockIdx.x * static_cast<long long>(COUNT_THREADS * COUNT_PER_THREAD) + threadIdx.x;
+#pragma unroll
+  for (int u = 0; u < COUNT_PER_THREAD; ++u) {
+    const long long i = i0 + u * COUNT_THREADS;
+    if (i >= n) break;
+    int id = ids[i];
+    if (id < 0 || id >= E) {
+      report(status, KS_BAD_ARGUMENT);
+      id = 0;
+    }
+    picks[i] = id;
+    atomicAdd(&hist[id], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += COUNT_THREADS)
+    if (hist[e]) atomicAdd(counts + e, hist[e]);
 }
 
 // One block. offsets[E+1] (padded to 128), tile_expert[max_tiles], cursor[E] = first row of each expert.
@@ -420,6 +449,16 @@ int ss_moe_route_bwd(const float* logits, long long ld, const int* ids, const fl
   if (T <= 0) return 0;
   moe_route_bwd_kernel<<<(T + 7) / 8, ROUTE_THREADS, 0, (cudaStream_t)stream>>>(logits, ld, ids, weights, dweights,
                                                                                 dlogits, T, E, k, renormalize);
+  return (int)cudaGetLastError();
+}
+
+// ids, picks: int32 [n]; counts: int32 [E].
+int ss_moe_count(const int* ids, long long n, int E, int* counts, int* picks, int* status, void* stream) {
+  if (E < 1 || E > MOE_MAX_E || n < 0) return -2;
+  cudaStream_t s = (cudaStream_t)stream;
+  cudaMemsetAsync(counts, 0, sizeof(int) * E, s);
+  const long long per = COUNT_THREADS * COUNT_PER_THREAD;
+  if (n > 0) moe_count_kernel<<<(int)((n + per - 1) / per), COUNT_THREADS, 0, s>>>(ids, n, E, counts, picks, status);
   return (int)cudaGetLastError();
 }
 

@@ -17,6 +17,7 @@ from . import _lib
 _c = _lib
 _lib.register("ss_moe_route", [_c.c_p, _c.c_ll, _c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_p,
                                _c.c_p, _c.c_p, _c.c_p])
+_lib.register("ss_moe_count", [_c.c_p, _c.c_ll, _c.c_int, _c.c_p, _c.c_p, _c.c_p, _c.c_p])
 _lib.register("ss_moe_layout", [_c.c_p, _c.c_p, _c.c_int, _c.c_int, _c.c_int, _c.c_p, _c.c_p,
                                 _c.c_int, _c.c_p, _c.c_p, _c.c_p, _c.c_int, _c.c_p])
 _lib.register("ss_moe_route_bwd", [_c.c_p, _c.c_ll, _c.c_p, _c.c_p, _c.c_p, _c.c_p, _c.c_int, _c.c_int, _c.c_int,
@@ -57,6 +58,18 @@ def route_bwd(logits: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, dwts: 
                                            dwts.data_ptr(), dlogits.data_ptr(), T, E, ids.shape[1],
                                            int(renormalize), _lib.stream_ptr()), "ss_moe_route_bwd")
     return dlogits
+
+
+def counted(ids: torch.Tensor, E: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Picks [T,k] of a routing made elsewhere -> (picks int32 [T,k] in range, counts int32 [E]), for ``Layout``. A pick outside
+    ``[0, E)`` is reported like a wait that gave up (``_lib.check_status``: bad argument) and counted for expert 0."""
+    if ids.dtype != torch.int32:
+        ids = ids.clamp(-1, E).to(torch.int32)
+    ids = ids.contiguous()
+    picks, counts = torch.empty_like(ids), torch.empty(E, dtype=torch.int32, device=ids.device)
+    _lib.check(_lib.lib().ss_moe_count(ids.data_ptr(), ids.numel(), E, counts.data_ptr(), picks.data_ptr(),
+                                       _lib.status_ptr(ids), _lib.stream_ptr()), "ss_moe_count")
+    return picks, counts
 
 
 class Layout:

@@ -201,3 +201,33 @@ def test_a_layer_of_more_picks_than_lanes():
     # activations, products and their gradients are stored in bf16, four of them in a chain, each off by 2^-8 of its value
     for got, exact in ((out, want), *((a, b.grad) for a, b in zip(grads, ref))):
         assert float((got.double() - exact.detach()).norm()) <= 4 * 2.0 ** -8 * float(exact.detach().norm())
+
+
+@pytest.mark.parametrize("T,k,E", [(1, 1, 1), (700, 3, 512), (8192, 8, 64), (0, 4, 8), (33, 40, 48)])
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_picks_made_elsewhere_are_counted(T, k, E, dtype):
+    from shadowspill_b200.ops import _lib, moe
+    ids = torch.randint(0, E, (T, k), generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).to(dtype)
+    picks, counts = moe.counted(ids, E)
+    assert torch.equal(picks, ids.int()) and torch.equal(counts.long(), torch.bincount(ids.reshape(-1).long(), minlength=E))
+    _lib.check_status()
+
+
+@pytest.mark.parametrize("bad", [-1, 8, 513, 2 ** 31 - 1, -2 ** 31])
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_a_pick_of_no_expert_is_reported(bad, dtype):
+    import shadowspill_b200.frontend.ops  # noqa: F401
+    from shadowspill_b200.ops import _lib
+    T, D, Fw, E, k = 40, 128, 128, 8, 2
+    h, w13, w2 = _rand(T, D, seed=1).bfloat16(), (_rand(E, 2 * Fw, D, seed=2) * 0.1).bfloat16(), (_rand(E, D, Fw, seed=3) * 0.1).bfloat16()
+    ids = torch.randint(0, E, (T, k), generator=torch.Generator(device=DEV).manual_seed(4), device=DEV).to(dtype)
+    w = torch.rand(T, k, device=DEV)
+    want = torch.ops.ss.moe_experts_routed(h, ids, w, w13, w2)
+    _lib.check_status()
+    wrong = ids.clone()
+    wrong[3, 1] = bad
+    torch.ops.ss.moe_experts_routed(h, wrong, w, w13, w2)
+    with pytest.raises(RuntimeError, match="bad argument"):
+        _lib.check_status()
+    assert torch.equal(torch.ops.ss.moe_experts_routed(h, ids, w, w13, w2), want)
+    _lib.check_status()
