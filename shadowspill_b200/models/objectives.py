@@ -18,7 +18,7 @@ objectives/head/execution.py:17-60; objectives/moe.py:4): ``shadowspill/cross_en
 """
 from __future__ import annotations
 
-from dataclasses import asdict, dataclass
+from dataclasses import asdict, dataclass, replace
 from typing import Any
 
 from ..ops.reference import PREFERENCE_KINDS
@@ -89,8 +89,7 @@ class Objective:
         if kind == "sum":
             head = Objective.from_component(config.get("head", COMPONENT_IDS["cross_entropy"]),
                                             **config.get("head_config", {}))
-            return Objective(head.kind, head.clip_ratio, head.reference_beta,
-                             float(config.get("moe_balance", 0.0)))
+            return replace(head, moe_balance_coef=float(config.get("moe_balance", 0.0)))
         if kind == "moe_balance":
             raise ValueError("moe_balance is only usable inside a sum")
         return Objective(kind, **config)

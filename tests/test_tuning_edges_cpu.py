@@ -33,3 +33,12 @@ def test_more_picks_than_experts_are_refused_on_the_cpu():
         with pytest.raises(ValueError):
             torch.ops.ss.select_experts(_rand(3, 8), torch.zeros(8), k, True, groups, keep, True, 1.0)
     assert R.select_experts(_rand(3, 8), 8)[0].shape == (3, 8)
+
+
+def test_a_sum_keeps_its_heads_settings():
+    from shadowspill_b200.models.objectives import Objective
+    settings = dict(preference_loss="ipo", preference_beta=0.5, average_logprobs=True, reference_free=True)
+    got = Objective.from_component("shadowspill/sum@1", head="shadowspill/preference@1", head_config=settings, moe_balance=0.01)
+    assert got == Objective("preference", moe_balance_coef=0.01, **settings) and got.extra_fields == ()
+    got = Objective.from_component("shadowspill/sum@1", head="shadowspill/clipped_policy@1", head_config={"clip_ratio": 0.1, "reference_beta": 0.3})
+    assert got == Objective("clipped_policy", clip_ratio=0.1, reference_beta=0.3)
