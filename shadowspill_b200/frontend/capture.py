@@ -163,8 +163,10 @@ class TrainingDescription:
         if self.frontend == "graph" or self.cfg.is_latent_attention:
             from .graph_stage import build_graph_stages, supports
             if self.cfg.is_latent_attention and not supports(self.cfg, self.lora, ep, self.objective):
-                raise ValueError(f"the {self.cfg.family} family is defined for the graph frontend only, which "
-                                 "does not cover expert parallelism or the router-balance term yet")
+                kind = getattr(self.objective, "kind", "cross_entropy")
+                raise ValueError(f"the {self.cfg.family} family is defined for the graph frontend only, which does not cover "
+                                 + (f"the {kind} objective" if kind != "cross_entropy" else
+                                    "expert parallelism, the router-balance term or this choice of adapters") + " yet")
             if supports(self.cfg, self.lora, ep, self.objective):
                 stages = build_graph_stages(self.cfg, self.geometry.microbatch_tokens, self.geometry.slots,
                                             self.dtype, self.grad_dtype, self.head_block_rows,

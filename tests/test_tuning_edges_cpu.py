@@ -42,3 +42,14 @@ def test_a_sum_keeps_its_heads_settings():
     assert got == Objective("preference", moe_balance_coef=0.01, **settings) and got.extra_fields == ()
     got = Objective.from_component("shadowspill/sum@1", head="shadowspill/clipped_policy@1", head_config={"clip_ratio": 0.1, "reference_beta": 0.3})
     assert got == Objective("clipped_policy", clip_ratio=0.1, reference_beta=0.3)
+
+
+def test_the_graph_only_family_names_the_objective_that_it_does_not_cover():
+    from shadowspill_b200.frontend.capture import BatchGeometry, StepDataOrdering, build_step
+    from shadowspill_b200.models.config import preset
+    from shadowspill_b200.models.objectives import Objective
+    geo = BatchGeometry(microbatch_tokens=256, n_microbatches=2, slots=16, mean_seqlen=64)
+    for ob, match in ((Objective("preference"), "the preference objective"), (Objective("clipped_policy"), "the clipped_policy objective"),
+                      (Objective(moe_balance_coef=0.01), "router-balance")):
+        with pytest.raises(ValueError, match=match):
+            build_step(preset("glm53-tiny"), geo, StepDataOrdering(), dtype=torch.float32, objective=ob)
