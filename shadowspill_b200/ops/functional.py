@@ -676,8 +676,9 @@ def adamw8_many_(tensors, *, lr, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0
         tables.clear()
         seen.clear()
 
+    for t in tensors:                       # all of them before the first is updated
+        _check_moments8(*t)
     for p, g, m, r, m_exp, r_exp, offset in tensors:
-        _check_moments8(p, g, m, r, m_exp, r_exp, offset)
         if not _cuda(p):
             reference.adamw8_(p, g, m, r, m_exp, r_exp, **hyper)
             continue

@@ -53,3 +53,14 @@ def test_the_graph_only_family_names_the_objective_that_it_does_not_cover():
                       (Objective(moe_balance_coef=0.01), "router-balance")):
         with pytest.raises(ValueError, match=match):
             build_step(preset("glm53-tiny"), geo, StepDataOrdering(), dtype=torch.float32, objective=ob)
+
+
+def test_an_update_that_is_refused_leaves_every_tensor_as_it_was():
+    from shadowspill_b200.ops import functional as F
+    good = [(torch.ones(300), torch.ones(300), *F.moments8(300), 0) for _ in range(2)]
+    for bad in ((torch.ones(8), torch.ones(7), *F.moments8(8), 0), (torch.ones(8), torch.ones(8), *F.moments8(8), 4),
+                (torch.ones(8, dtype=torch.float64), torch.ones(8), *F.moments8(8), 0)):
+        with pytest.raises((ValueError, TypeError)):
+            F.adamw8_many_([*good, bad], lr=0.1)
+        for p, _, m, r, m_exp, r_exp, _ in good:
+            assert float((p - 1).abs().max()) == 0.0 and not any(int(x.view(torch.uint8).sum()) for x in (m, r, m_exp, r_exp))
