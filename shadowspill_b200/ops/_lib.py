@@ -47,7 +47,7 @@ _SIGNATURES = {
                     c_ull, c_int, c_int, c_p],
     "ss_adamw_sr_many": [c_p, c_int, c_f, c_f, c_f, c_f, c_f, c_int, c_f, c_ull, c_int, c_int, c_p],
     "ss_adamw_f32": [c_p, c_p, c_p, c_p, c_ll, c_f, c_f, c_f, c_f, c_f, c_int, c_f, c_p],
-    "ss_adamw8_many": [c_p, c_int, c_int, c_int, c_p, c_int, c_ll, c_int, c_int, c_p],
+    "ss_adamw8_many": [c_p, c_int, c_int, c_int, c_p, c_int, c_ll, c_int, c_int, c_p, c_p],
     "ss_preference": [c_p, c_int, c_ll, c_p, c_p, c_p, c_int, c_int, c_int, c_p, c_f, c_int, c_f, c_int, c_f, c_p, c_p, c_p,
                       c_p, c_ll, c_p, c_p],
     "ss_sumsq": [c_p, c_ll, c_p, c_p, c_int, c_p],
@@ -164,16 +164,16 @@ def check_status(device: torch.device | int | None = None) -> None:
 
 # kernels launched by one successful call of each launcher (attention backward:
 # delta + dQ + dKV; sum of squares: partials + final; preference loss: rows + gradient). What only clears a call's
-# counters is not counted.
+# counters is not counted, nor are calls without rows.
 _KERNELS_PER_CALL = {"ss_attn_bwd": 3, "ss_attn_bwd_g": 3, "ss_sumsq": 2, "ss_preference with its gradient": 2}
 _by_entry: dict[str, int] = {}
 
 
-def check(rc: int, what: str) -> None:
-    """Raises on a failed launcher; counts the kernels a successful one enqueued."""
+def check(rc: int, what: str, kernels: int | None = None) -> None:
+    """Raises on a failed launcher; counts the kernels a successful one enqueued (``kernels``: where the call decides)."""
     if rc != 0:
         raise RuntimeError(f"{what} failed with code {rc}")
-    n = _KERNELS_PER_CALL.get(what, 1)
+    n = _KERNELS_PER_CALL.get(what, 1) if kernels is None else kernels
     _by_entry[what] = _by_entry.get(what, 0) + n
 
 

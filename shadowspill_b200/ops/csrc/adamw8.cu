@@ -473,9 +473,10 @@ using namespace ss;
 
 // `tensors`: eight values per tensor, {p, g, m, r, m_exp, r_exp, elements, offset}, and `hyper`, {lr, beta1, beta2, eps, weight decay,
 // gradient scale}, in host memory, read before the call returns. No element is in two tensors; all parameters are of
-// one type, and all gradients.
+// one type, and all gradients. `launched` receives the number of kernels: one to 48 tensors, and to 48 off the boundaries of their pieces.
 int ss_adamw8_many(const long long* tensors, int count, int p_f32, int g_f32, const double* hyper, int step, long long seed,
-                   int sr_param, int sr_state, void* stream) {
+                   int sr_param, int sr_state, int* launched, void* stream) {
+  *launched = 0;
   const double lr = hyper[0], beta1 = hyper[1], beta2 = hyper[2], eps = hyper[3], weight_decay = hyper[4], grad_scale = hyper[5];
   if (step < 1) return -2;
   long long total = 0;
@@ -533,6 +534,7 @@ int ss_adamw8_many(const long long* tensors, int count, int p_f32, int g_f32, co
                           : (g_f32 ? launch8<bf16, float, STAGED>(tab, a, n, sr_param, sr_state, s)
                                    : launch8<bf16, bf16, STAGED>(tab, a, n, sr_param, sr_state, s));
       if (e) return e;
+      ++*launched;
     }
     return 0;
   };

@@ -48,16 +48,20 @@ long long g_launched[ENTRIES];           // under the GIL
 
 struct Failed { const char* what; int rc; };
 
+// `kernels`: how many a successful call enqueues; a launcher may write it.
 template <class F, class... A>
-void launch(Entry e, F* entry, A... args) {
+void launch_some(Entry e, const int& kernels, F* entry, A... args) {
   int rc;
   {
     NoGil free;
     rc = entry(args...);
   }
   if (rc) throw Failed{kNames[e], rc};
-  // delta, dQ, dK and dV; rows and gradient (as _lib counts them)
-  g_launched[e] += e == ATTN_BWD ? 3 : e == PREFERENCE_GRAD ? 2 : 1;
+  g_launched[e] += kernels;
+}
+template <class F, class... A>
+void launch(Entry e, F* entry, A... args) {
+  launch_some(e, 1, entry, args...);
 }
 
 const at::Tensor& tensor(PyObject* o) {
@@ -323,7 +327,7 @@ PyObject* attention_bwd(PyObject*, PyObject* const* v, Py_ssize_t n) {
       ld[i] = rows3(g[i], T, heads[i], dh);
     }
     at::Tensor delta = empty({H, T}, c.f32);          // kernel scratch
-    launch(ATTN_BWD, ss_attn_bwd_g, q.data_ptr(), k.data_ptr(), vv.data_ptr(), out.data_ptr(),
+    launch_some(ATTN_BWD, 3, ss_attn_bwd_g, q.data_ptr(), k.data_ptr(), vv.data_ptr(), out.data_ptr(),
                                  static_cast<const float*>(lse.data_ptr()), dout.data_ptr(), g[0].data_ptr(),
                                  g[1].data_ptr(), g[2].data_ptr(), static_cast<const int*>(cu.data_ptr()),
                                  static_cast<float*>(delta.data_ptr()), cu.numel() - 1, T, H, Hk, dh, ldq, ldk, ldv, ldo,
@@ -388,7 +392,7 @@ PyObject* select_experts_bwd(PyObject*, PyObject* const* v, Py_ssize_t n) {
     const int64_t T = x.size(0), E = x.size(1), k = ids.size(1), sigmoid = integer(v[3]);
     want((sigmoid == 0 || sigmoid == 1) && E >= 1 && E <= 512 && k >= 1 && k <= E);
     at::Tensor out = empty({T, E}, x.options().requires_grad(false));
-    launch(SELECT_BWD, ss_select_experts_bwd, x.data_ptr(), !f32, pitch(x), static_cast<const int*>(ids.data_ptr()),
+    launch_some(SELECT_BWD, T != 0, ss_select_experts_bwd, x.data_ptr(), !f32, pitch(x), static_cast<const int*>(ids.data_ptr()),
            static_cast<const float*>(dw.data_ptr()), T, E, k, sigmoid, v[4] == Py_True, static_cast<float>(number(v[5])),
            out.data_ptr(), stream);
     return wrap(std::move(out));
@@ -426,7 +430,7 @@ PyObject* preference(PyObject*, PyObject* const* v, Py_ssize_t n) {
     at::Tensor work = empty({6 * R + 3 * S + 1 + (logp == nullptr ? R : 0)}, options);
     float* w = static_cast<float*>(work.data_ptr());
     if (logp == nullptr) logp = w + 6 * R + 3 * S + 1;
-    launch(grad == nullptr ? PREFERENCE : PREFERENCE_GRAD, ss_preference, x.data_ptr(), f32, pitch(x),
+    launch_some(grad == nullptr ? PREFERENCE : PREFERENCE_GRAD, grad == nullptr || R == 0 ? 1 : 2, ss_preference, x.data_ptr(), f32, pitch(x),
            static_cast<const long long*>(targets.data_ptr()), weights, static_cast<const int*>(cu.data_ptr()), R, V, S / 2, ref,
            static_cast<float>(beta), kind, static_cast<float>(smoothing), v[8] == Py_True, static_cast<float>(number(v[10])), logp, sums,
            loss, grad == nullptr ? nullptr : grad->data_ptr(), grad == nullptr ? 0 : pitch(*grad), w, stream);
@@ -476,8 +480,9 @@ PyObject* adamw8_many(PyObject*, PyObject* const* v, Py_ssize_t n) {
     for (int j = 0; j < 6; ++j) hyper[j] = number(PyTuple_GET_ITEM(v[1], j));
     const long long step = integer(v[2]);
     want(step >= 1 && step <= INT_MAX && hyper[3] >= 1e-16);
-    launch(ADAMW8, ss_adamw8_many, table.data(), count, types[0] == at::kFloat, types[1] == at::kFloat, hyper, step, integer(v[3]),
-           v[4] == Py_True, v[5] == Py_True, stream);
+    int kernels = 0;
+    launch_some(ADAMW8, kernels, ss_adamw8_many, table.data(), count, types[0] == at::kFloat, types[1] == at::kFloat, hyper, step, integer(v[3]),
+                v[4] == Py_True, v[5] == Py_True, &kernels, stream);
     Py_RETURN_NONE;
   });
 }

@@ -49,5 +49,5 @@ int ss_preference(const void* logits, int fp32_logits, long long ld, const long 
                   void* stream);
 // adamw8.cu
 int ss_adamw8_many(const long long* tensors, int count, int p_f32, int g_f32, const double* hyper, int step, long long seed,
-                   int sr_param, int sr_state, void* stream);
+                   int sr_param, int sr_state, int* launched, void* stream);
 }

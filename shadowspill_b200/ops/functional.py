@@ -542,7 +542,7 @@ def preference_(logits, targets, weights, cu_seqlens, loss_sum, *, beta=0.1, kin
             cu_seqlens.data_ptr(), R, V, S // 2, _ptr(ref_logp), float(beta), reference.PREFERENCE_KINDS.index(kind),
             float(label_smoothing), int(average), float(grad_scale), lp.data_ptr(), _ptr(sums), loss_sum.data_ptr(), _ptr(out),
             0 if out is None else max(out.stride(0), V), work.data_ptr(), _lib.stream_ptr()),
-            "ss_preference" if out is None else "ss_preference with its gradient")
+            "ss_preference" if out is None else "ss_preference with its gradient", None if R else 1)
     return loss_sum
 
 
@@ -669,10 +669,12 @@ def adamw8_many_(tensors, *, lr, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0
     def flush():
         for (_, p_dtype, g_dtype), (where, table) in tables.items():
             with _device_of(where):
+                kernels = ctypes.c_int()
                 _lib.check(_lib.lib().ss_adamw8_many(
                     (ctypes.c_longlong * len(table))(*table), len(table) // 8, int(p_dtype == torch.float32),
                     int(g_dtype == torch.float32), (ctypes.c_double * 6)(lr, beta1, beta2, eps, weight_decay, grad_scale), step,
-                    seed, int(stochastic_param), int(stochastic_state), _lib.stream_ptr()), "ss_adamw8_many")
+                    seed, int(stochastic_param), int(stochastic_state), ctypes.addressof(kernels), _lib.stream_ptr()),
+                    "ss_adamw8_many", kernels.value)
         tables.clear()
         seen.clear()
 

@@ -95,5 +95,5 @@ def select_experts_bwd(logits: torch.Tensor, ids: torch.Tensor, dweights: torch.
         _lib.check(_lib.lib().ss_select_experts_bwd(
             logits.data_ptr(), int(logits.dtype == torch.bfloat16), max(logits.stride(0), E), ids.data_ptr(),
             dweights.data_ptr(), T, E, ids.shape[1], _SIGMOID[scoring], int(renormalize), float(scale), out.data_ptr(),
-            _lib.stream_ptr()), "ss_select_experts_bwd")
+            _lib.stream_ptr()), "ss_select_experts_bwd", int(T > 0))
     return out
