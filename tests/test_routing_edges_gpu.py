@@ -231,3 +231,24 @@ def test_a_pick_of_no_expert_is_reported(bad, dtype):
         _lib.check_status()
     assert torch.equal(torch.ops.ss.moe_experts_routed(h, ids, w, w13, w2), want)
     _lib.check_status()
+
+
+# lanes to a token and experts to a lane by the launcher's rule: 16 and 16 by logits alone and with a bias, 32 and 4, 32 and 8
+@pytest.mark.parametrize("E,k,bias,groups,keep", [(256, 8, False, 1, 1), (129, 8, False, 1, 1), (200, 1, False, 1, 1), (256, 5, True, 1, 1),
+                                                  (131, 3, True, 1, 1), (256, 2, True, 8, 8), (128, 9, False, 1, 1), (66, 32, False, 1, 1),
+                                                  (256, 9, False, 1, 1), (129, 32, False, 1, 1), (240, 20, False, 1, 1)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_picks_of_every_kernel(E, k, bias, groups, keep, scoring, dtype):
+    g = torch.Generator(device=DEV).manual_seed(E + k)
+    rough = torch.randint(-3, 4, (300, E), generator=g, device=DEV).float() * 0.5           # ties
+    near = _rand(300, 1, seed=1) + torch.randint(-4, 5, (300, E), generator=g, device=DEV) * 2.0 ** -22
+    b = _rand(E, seed=3) * 0.1 if bias else None
+    for x in (_rand(1003, E, seed=2) * 1.5, rough, near):
+        x = x.to(dtype)
+        for renormalize in (True, False):
+            ids, w, counts = routing.select_experts(x, k, scoring=scoring, bias=b, groups=groups, keep_groups=keep, renormalize=renormalize)
+            want = R.select_experts(x, k, scoring, b, groups, keep, renormalize)
+            assert torch.equal(ids, want[0]) and torch.equal(counts, want[2])
+            # as in the tests of softmax and sigmoid weights, arguments up to 16; sums of up to 32 renormalised
+            assert bool(((w - want[1]).abs() <= 2 * (8 + 18) * STEP * want[1]).all())
