@@ -320,7 +320,7 @@ __device__ void finish_empty(const Rows& rows, const Work& work, float* sums, fl
 }
 
 __global__ void clear_counters_kernel(int* words, int n) {
-  chain_wait();
+  chain_wait();                                  // ahead of the release: what comes behind reads its inputs without a wait of its own
   chain_release();
   for (int i = threadIdx.x; i < n; i += blockDim.x) words[i] = 0;
 }
@@ -339,7 +339,7 @@ preference_rows_kernel(const L* logits, long long ld, bool aligned, Rows rows, P
   const int rank = Team<TEAM>::rank(), row = Team<TEAM>::row();
   double (*red)[WARPS] = red_of[threadIdx.x / TEAM];
   // This kernel starts beside the one that clears its counters, which has waited for all work before; the
-  // counters alone have to be waited for.
+  // counters alone have to be waited for (chained_launch.cuh: the exception). Every block has a row up to the R-th and so waits.
   if (row > rows.R) return;
   if (row == rows.R) {
     chain_wait();

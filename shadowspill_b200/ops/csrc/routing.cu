@@ -261,7 +261,7 @@ template <int LANES, int PER, bool LOGITS, class L>
 __global__ void __launch_bounds__(RT_THREADS, rt_resident(PER))
 select_experts_kernel(const L* logits, bool vectors, bool bias_vectors, RouteArgs a, int* ids, float* weights, int* counts) {
   // Several blocks count behind the kernel that clears the counts, which lets this one start beside it, after its own wait for
-  // all work before: what it waits for itself is the cleared counts alone, at the end.
+  // all work before: what it waits for itself is the cleared counts alone, at the end (chained_launch.cuh: the exception).
   const bool alone = gridDim.x == 1;
   if (alone) chain_wait();
   constexpr int TOKENS = 32 / LANES;             // of a warp
@@ -622,7 +622,7 @@ select_many_kernel(const L* logits, RouteArgs a, int* ids, float* weights, int* 
 }
 
 __global__ void clear_counts_kernel(int* counts, int E) {
-  chain_wait();
+  chain_wait();                                  // ahead of the release: what comes behind reads inputs without a wait of its own
   chain_release();
   for (int e = threadIdx.x; e < E; e += blockDim.x) counts[e] = 0;
 }
