@@ -24,6 +24,7 @@
 
 #include "chained_launch.cuh"
 #include "launchers.h"
+#include "philox.cuh"
 
 namespace ss {
 namespace {
@@ -47,19 +48,6 @@ struct Args8 {
   float beta1, beta2, c1, c2, eps, keep, minus_lr, inv_bias2, grad_scale, one;   // minus_lr: with the first bias correction
   unsigned long long seed;
 };
-
-// Philox4x32-10, as the other update kernels use it.
-__device__ __forceinline__ uint4 philox(uint4 c, uint2 key) {
-#pragma unroll
-  for (int i = 0; i < 10; ++i) {
-    const uint32_t h0 = __umulhi(0xD2511F53u, c.x), l0 = 0xD2511F53u * c.x;
-    const uint32_t h1 = __umulhi(0xCD9E8D57u, c.z), l1 = 0xCD9E8D57u * c.z;
-    c = make_uint4(h1 ^ c.y ^ key.x, l1, h0 ^ c.w ^ key.y, l0);
-    key.x += 0x9E3779B9u;
-    key.y += 0xBB67AE85u;
-  }
-  return c;
-}
 
 // The eight elements of a lane, by pairs: two fp32 operations to an instruction. Each operation is rounded by itself.
 struct Eight {
@@ -201,8 +189,8 @@ __device__ __forceinline__ void update8(Read8<P, G>& x, const Args8& a, unsigned
     const unsigned long long at = element >> 3;
     const uint2 key = make_uint2(static_cast<uint32_t>(a.seed), static_cast<uint32_t>(a.seed >> 32));
     const uint32_t c0 = static_cast<uint32_t>(at), c1 = static_cast<uint32_t>(at >> 32);
-    if (SR_PARAM) random = philox(make_uint4(c0, c1, 0u, 0x3838u), key);
-    if (SR_STATE) rs = philox(make_uint4(c0, c1, 1u, 0x3838u), key);
+    if (SR_PARAM) random = philox4x32(make_uint4(c0, c1, 0u, 0x3838u), key);
+    if (SR_STATE) rs = philox4x32(make_uint4(c0, c1, 1u, 0x3838u), key);
   }
   const float m_inv = unit_of(254 - x.m_exp), r_inv = unit_of(254 - x.r_exp);
   constexpr float FLOOR = 0.001953125f;                        // code 1

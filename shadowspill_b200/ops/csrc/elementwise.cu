@@ -10,6 +10,7 @@
 #include <stdint.h>
 
 #include "chained_launch.cuh"
+#include "philox.cuh"
 #include "swiglu_math.cuh"
 #include "launchers.h"
 
@@ -446,19 +447,7 @@ take_rows_kernel(const bf16* x, long long ldx, const int* index, bf16* out, long
 }
 
 // =============================================================== AdamW with stochastic rounding
-// Philox4x32-10 counter RNG: (seed, step) key, element index counter.
-__device__ __forceinline__ uint4 philox4x32(uint4 ctr, uint2 key) {
-  const uint32_t M0 = 0xD2511F53u, M1 = 0xCD9E8D57u, W0 = 0x9E3779B9u, W1 = 0xBB67AE85u;
-#pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const uint32_t hi0 = __umulhi(M0, ctr.x), lo0 = M0 * ctr.x;
-    const uint32_t hi1 = __umulhi(M1, ctr.z), lo1 = M1 * ctr.z;
-    ctr = make_uint4(hi1 ^ ctr.y ^ key.x, lo1, hi0 ^ ctr.w ^ key.y, lo0);
-    key.x += W0;
-    key.y += W1;
-  }
-  return ctr;
-}
+// Random bits by (seed, step) key and element index counter.
 struct AdamWArgs {
   float lr, beta1, beta2, eps, weight_decay, bias1, bias2, grad_scale;
   unsigned long long seed;

@@ -25,6 +25,8 @@
 #include <stdint.h>
 #include <stdlib.h>
 
+#include "philox.cuh"
+
 namespace ss {
 
 constexpr int MAX_RANKS = 16;
@@ -111,17 +113,6 @@ __global__ void peer_allgather_kernel(PeerPtrs shards, uint8_t* __restrict__ ful
 }
 
 // ---- AdamW pieces (same arithmetic and RNG as adamw_sr_kernel in elementwise.cu)
-__device__ __forceinline__ uint4 philox(uint4 ctr, uint2 key) {
-  const uint32_t M0 = 0xD2511F53u, M1 = 0xCD9E8D57u, W0 = 0x9E3779B9u, W1 = 0xBB67AE85u;
-#pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const uint32_t hi0 = __umulhi(M0, ctr.x), lo0 = M0 * ctr.x;
-    const uint32_t hi1 = __umulhi(M1, ctr.z), lo1 = M1 * ctr.z;
-    ctr = make_uint4(hi1 ^ ctr.y ^ key.x, lo1, hi0 ^ ctr.w ^ key.y, lo0);
-    key.x += W0; key.y += W1;
-  }
-  return ctr;
-}
 __device__ __forceinline__ uint16_t sr16(float f, uint32_t rnd) {
   uint32_t u = __float_as_uint(f);
   if ((u & 0x7f800000u) == 0x7f800000u) return static_cast<uint16_t>(u >> 16);
@@ -259,7 +250,7 @@ __global__ void rs_adamw_kernel(PeerPtrs grads, const __nv_bfloat16* __restrict_
     uint4 r[3];
 #pragma unroll
     for (int k = 0; k < 3; ++k)
-      r[k] = philox(make_uint4(static_cast<uint32_t>(gidx >> 3), static_cast<uint32_t>(gidx >> 35),
+      r[k] = philox4x32(make_uint4(static_cast<uint32_t>(gidx >> 3), static_cast<uint32_t>(gidx >> 35),
                                static_cast<uint32_t>(k), 0x5353u), key);
     const uint32_t rw[12] = {r[0].x, r[0].y, r[0].z, r[0].w, r[1].x, r[1].y,
                              r[1].z, r[1].w, r[2].x, r[2].y, r[2].z, r[2].w};
