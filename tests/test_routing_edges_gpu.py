@@ -252,3 +252,16 @@ def test_picks_of_every_kernel(E, k, bias, groups, keep, scoring, dtype):
             assert torch.equal(ids, want[0]) and torch.equal(counts, want[2])
             # as in the tests of softmax and sigmoid weights, arguments up to 16; sums of up to 32 renormalised
             assert bool(((w - want[1]).abs() <= 2 * (8 + 18) * STEP * want[1]).all())
+
+
+def test_an_eager_backward_pass_that_would_wait_for_itself_is_refused():
+    import shadowspill_b200.frontend.ops  # noqa: F401
+    T, D, Fw, E, k = 16, 128, 128, 8, 2
+    h, w13, w2 = _rand(T, D, seed=1).bfloat16(), (_rand(E, 2 * Fw, D, seed=2) * 0.1).bfloat16(), (_rand(E, D, Fw, seed=3) * 0.1).bfloat16()
+    ids, w = torch.ops.ss.select_experts(_rand(T, E, seed=4), _rand(E, seed=5), k, True, 1, 1, True, 1.0)
+    for leaf in (h, w, w13):
+        leaf.requires_grad_(True)
+    out = torch.ops.ss.moe_experts_routed(h, ids, w, w13, w2)
+    with pytest.raises(RuntimeError, match="exported stages"):
+        out.sum().backward()
+    assert len(torch.ops.ss.moe_experts_routed_bwd(h.detach(), ids, w.detach(), w13.detach(), w2, torch.ones_like(h), True)) == 4
