@@ -471,7 +471,8 @@ class HeadLossStage(Stage):
         return (min(T, self._block(T)) * c.vocab_size + 2 * T * c.d_model) * itemsize
 
     def _block(self, T):
-        """Rows of logits formed at once: all of them for pairs, whose gradients wait for both of their sequences."""
+        """Rows of logits formed at once: all of them for pairs, whose gradients wait for both of their sequences; ``block_rows`` (and so
+        a session's ``head_chunks``) has no effect there."""
         return max(T, 1) if self.objective.kind == "preference" else self.block_rows
 
     def flops(self, T, mean_seqlen):

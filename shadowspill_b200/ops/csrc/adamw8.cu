@@ -11,8 +11,9 @@
 // The new moments are formed in fp32, one rounding to an operation (no contraction), so that the codes rounded to nearest
 // are those of the same operations anywhere else; the parameter's step uses them before they are rounded.
 //
-// Bound by memory: 10 bytes and 1/64 an element in bf16, 218 M elements in 330 us, 6.6 TB/s, with the moments and parameters rounded to nearest (fp32: 16 bytes, 527 us); with
-// random bits 418 us, three Philox calls to eight elements, where bf16 moments take 555.
+// Bound by memory: 10 bytes and 1/64 an element in bf16, 218 M elements in 334 us, 6.5 TB/s (336 to 356 a call, one behind the other), with the moments and
+// parameters rounded to nearest (fp32: 16 bytes, 530 us); with random bits, as by default, 432 us, two Philox calls to eight elements, where bf16
+// moments take 575.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
@@ -241,7 +242,7 @@ template <class P, class G> struct Ring8 {
   static constexpr int STAGE = 32 * (16 * P16 + 16 * G16 + 16), STAGES = 48 * 1024 / A8_WARPS / STAGE;
 };
 // STAGED: tensors off the boundaries of their pieces. Neighbouring elements go by neighbouring lanes, and through shared memory to the eight
-// of a lane and back: 50 M bf16 elements, one element off, 156 us (by each lane's elements 303, on the boundaries 85). A kernel of its own: with
+// of a lane and back: 50 M bf16 elements, one element off, 186 us (on the boundaries 109; by each lane's elements 3.7 times that). A kernel of its own: with
 // this in the other one a layer of 218 M elements took 376 us instead of 361.
 template <class P, class G, bool SR_PARAM, bool SR_STATE, bool STAGED>
 __global__ void __launch_bounds__(A8_THREADS, 3)

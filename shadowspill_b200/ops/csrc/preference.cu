@@ -8,8 +8,8 @@
 //
 // A row's gradient needs every row of its pair first, so the block is read twice: once for the rows' statistics, where the last row of a
 // pair to be done forms the pair's loss and slopes, once for the gradient. Both are bound by memory where the block is large: 4,096 rows of
-// 128,256 bf16 words, 70 % of them scored, take 418 us of which 388 are two reads and a write at the copy rate; 24 rows of 4,096
-// are three launches, 15 us.
+// 128,256 bf16 words, 70 % of them scored, take 418 to 430 us of which 388 are two reads and a write at the copy rate; 24 rows of 4,096
+// are three launches, 15 to 17 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <float.h>
@@ -445,8 +445,8 @@ preference_rows_kernel(const L* logits, long long ld, bool aligned, Rows rows, P
 // From the last row to the first: the rows read last are still in the L2. Nothing is summed here, so a thread may have any elements: the pieces
 // on the row's 16-byte boundaries and the few elements before and behind them, stored by element where the
 // gradient's boundaries lie elsewhere. Bound by memory: 1.05 GB written and 0.74 read in 272 us, 6.5 TB/s (4,096 rows of 128,256 words, 70 % scored).
-// 4,096 rows of 50,257 words, whole calls: 271 us, by element from the row's start 616; of 50,256 words 229. (The choice at the
-// store stays in the loop: without it a thread's four stores leave together, 243 us.)
+// 4,096 rows of 50,257 words, whole calls, 70 % scored: 243 us, by element from the row's start 2.3 times that; of 50,256 words 194. (The choice at the
+// store stays in the loop: without it a thread's four stores leave together, 6 % slower.)
 template <class L, int TEAM>
 __global__ void __launch_bounds__(Team<TEAM>::BLOCK)
 preference_grad_kernel(const L* logits, long long ld, const long long* targets, Work work, int R, int V, L* grad, long long ldg) {

@@ -248,9 +248,10 @@ __device__ __forceinline__ void load_row(const L* row, int first, int E, bool ve
   for (int i = 0; i < PER; ++i) v[i] = first + i < E ? load_logit(row + first + i) : -INFINITY;
 }
 
-// LANES to a token, PER consecutive experts to a lane. Bound by instructions: 8,192 tokens of 64 experts take 9 us, of 256
-// with a bias 19, and 65,537 of 512 in groups 128 us, 1,300 instructions a token with 60 % of the issue slots
-// used; their memory would take 0.5, 1.4 and 11.
+// LANES to a token, PER consecutive experts to a lane. Bound by instructions: 8,192 tokens of 64 experts take 8 us, of 256
+// with a bias 19, and 65,537 of 512 in groups 124 us, 1,300 instructions a token with 60 % of the issue slots
+// used; their memory would take 0.5, 1.4 and 11. At the registers that eight (seven) blocks an SM leave, the kernels that form keys spill
+// 84 to 220 bytes a thread, most of it around the rare paths.
 //
 // The k-th largest of the lanes' own maxima bounds the k-th largest key from below: the keys from it on, a dozen where k
 // is 8, are gathered by one place to a lane and sorted. Where they are more than the lanes (one token in twenty for k = 8 of 16

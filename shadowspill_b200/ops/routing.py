@@ -42,7 +42,7 @@ def select_experts(logits: torch.Tensor, k: int, *, scoring: str = "softmax", bi
     -inf or NaN come last, so that the ids of a token are always ``k`` different experts. The weights are the picks' scores
     (without the bias), divided by their sum (+ 1e-20) if ``renormalize``, times ``scale``; a token whose logits are all -inf
     gets weights of zero under softmax, one with a NaN or +inf gets NaN. At most 512 experts; ``k`` has no bound of its own (above 32 the
-    picks are made one by one in 64 bits, five times as long)."""
+    picks are made one by one in 64 bits, which takes several times as long)."""
     host = F._host(logits)
     if host is not None:
         got = host.select_experts(logits, k, _SIGMOID.get(scoring, -1), bias, groups, keep_groups, bool(renormalize), scale)
