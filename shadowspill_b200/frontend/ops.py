@@ -38,7 +38,7 @@ def _autograd_elsewhere(fn, inputs: tuple[Tensor, ...], grad_out: Tensor) -> tup
     kernel of its own on this device (the CPU forms of the sequence-mixer pieces). The body of a
     custom operator runs below the autograd dispatch keys, where nothing records a graph; that
     exclusion is thread-local, so the differentiation runs on a helper thread."""
-    if grad_out.is_cuda and torch._C._current_graph_task_id() != -1:
+    if grad_out.is_cuda and torch._C._current_graph_task_id() != -1 and torch._C._is_multithreading_enabled():
         # the helper's differentiation goes to the device's autograd thread, which is the one that would wait for it here
         raise RuntimeError("this operator's gradient on the GPU is for exported stages, which call its backward operator themselves: "
                            "inside loss.backward() it would wait for itself")

@@ -264,4 +264,7 @@ def test_an_eager_backward_pass_that_would_wait_for_itself_is_refused():
     out = torch.ops.ss.moe_experts_routed(h, ids, w, w13, w2)
     with pytest.raises(RuntimeError, match="exported stages"):
         out.sum().backward()
+    with torch.autograd.set_multithreading_enabled(False):       # in the caller's thread: the helper has the device's to itself
+        torch.ops.ss.moe_experts_routed(h, ids, w, w13, w2).sum().backward()
+    assert bool(torch.isfinite(h.grad).all()) and float(h.grad.abs().max()) > 0
     assert len(torch.ops.ss.moe_experts_routed_bwd(h.detach(), ids, w.detach(), w13.detach(), w2, torch.ones_like(h), True)) == 4
