@@ -64,7 +64,7 @@ def counted(ids: torch.Tensor, E: int) -> tuple[torch.Tensor, torch.Tensor]:
     """Picks [T,k] of a routing made elsewhere -> (picks int32 [T,k] in range, counts int32 [E]), for ``Layout``. A pick outside
     ``[0, E)`` is reported like a wait that gave up (``_lib.check_status``: bad argument) and counted for expert 0."""
     if ids.dtype != torch.int32:
-        ids = ids.clamp(-1, E).to(torch.int32)
+        ids = ids.long().clamp(-1, E).to(torch.int32)
     ids = ids.contiguous()
     picks, counts = torch.empty_like(ids), torch.empty(E, dtype=torch.int32, device=ids.device)
     _lib.check(_lib.lib().ss_moe_count(ids.data_ptr(), ids.numel(), E, counts.data_ptr(), picks.data_ptr(),
