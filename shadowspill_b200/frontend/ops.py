@@ -825,8 +825,9 @@ def select_experts(logits: Tensor, bias: Tensor, k: int, sigmoid: bool, groups: 
     from ..ops import routing
     scoring = "sigmoid" if sigmoid else "softmax"
     if not F._cuda(logits):
-        if not 1 <= k <= keep_groups * (logits.shape[1] // groups):
-            raise ValueError(f"cannot pick {k} of {keep_groups * (logits.shape[1] // groups)} experts")
+        E = logits.shape[1]
+        if not (1 <= keep_groups <= groups and E % groups == 0 and 1 <= k <= keep_groups * (E // groups)):
+            raise ValueError(f"cannot pick {k} of {E} experts in {groups} groups of which {keep_groups} are kept")
         ids, wts, _ = reference.select_experts(logits, k, scoring, bias, groups, keep_groups, renorm, scale)
         return ids, wts
     ids, wts, _ = routing.select_experts(logits, k, scoring=scoring, bias=bias, groups=groups,

@@ -29,7 +29,7 @@ def test_layers_of_any_number_of_experts_route_on_the_cpu(E, k, sigmoid):
 
 def test_more_picks_than_experts_are_refused_on_the_cpu():
     import shadowspill_b200.frontend.ops  # noqa: F401
-    for k, groups, keep in ((9, 1, 1), (0, 1, 1), (5, 4, 2)):
+    for k, groups, keep in ((9, 1, 1), (0, 1, 1), (5, 4, 2), (1, 3, 1), (1, 2, 3), (1, 2, 0)):
         with pytest.raises(ValueError):
             torch.ops.ss.select_experts(_rand(3, 8), torch.zeros(8), k, True, groups, keep, True, 1.0)
     assert R.select_experts(_rand(3, 8), 8)[0].shape == (3, 8)
